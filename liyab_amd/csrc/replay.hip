@@ -147,6 +147,10 @@ static const Entry kEntries[] = {
     LIYAB_ENTRY(liyab_scan_steps),
     LIYAB_ENTRY(liyab_selective_scan),
     LIYAB_ENTRY(liyab_selective_single),
+    LIYAB_ENTRY(liyab_mx_rows),
+    LIYAB_ENTRY(liyab_mx_glu),
+    LIYAB_ENTRY(liyab_mx_norm),
+    LIYAB_ENTRY(liyab_mx_product),
 };
 constexpr int kNumEntries = static_cast<int>(sizeof(kEntries) / sizeof(kEntries[0]));
 

@@ -149,6 +149,14 @@ _SIGNATURES = {
                              c_int, P, P, P],
     "liyab_selective_single": [P, c_int, P, P, c_int64, c_int, P, P, P, c_int64, P, P, P, c_int64, c_int, P, c_int64, c_int, P, P, P, c_int, c_int,
                                c_int, P],
+    "liyab_mx_quantize": [P, P, c_int, c_int64, c_int, c_int, P],
+    "liyab_mx_pack": [P, P, c_int64, P, c_int64, c_int, c_int, P],
+    "liyab_mx_dense": [P, c_int, c_int64, P, c_int, c_int, P],
+    "liyab_mx_rows": [P, c_int64, P, c_int64, P, c_int, c_int64, c_int, c_int, P],
+    "liyab_mx_glu": [P, c_int64, P, c_int64, P, c_int64, c_int, c_int, c_int, c_float, c_float, c_float, P],
+    "liyab_mx_norm": [P, c_int64, P, c_int64, P, P, c_int, P, P, P, c_float, c_int, c_int, c_int, P],
+    "liyab_mx_align": [P, c_int, P, c_int64, c_int, c_int, c_int, P],
+    "liyab_mx_product": [P, c_int64, P, c_int64, c_int, P, c_int, c_int, c_int, _EPI_PTR, P],
 }
 
 
@@ -231,6 +239,12 @@ def _encoders(name: str):
                          "address" if t is P else "int")
         hit = _entries[name] = (index, kinds) if index >= 0 and n.value == len(kinds) and "double" not in kinds else (-1, kinds)
     return hit
+
+
+def not_recordable() -> None:
+    """Says that the launches that follow use memory which is theirs alone: a list being recorded is of no use then."""
+    global _recording_whole
+    _recording_whole = False
 
 
 def _record(name: str, args) -> None:

@@ -1,0 +1,56 @@
+"""Microscaling formats without a GPU: the plain implementation's own numbers, and what the operators refuse."""
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import plain_mx
+from liyab_amd.errors import KernelError
+from liyab_amd.kernels import mx
+
+
+def test_numbers_of_the_formats():
+    assert plain_mx.E4M3[-1] == 448 and plain_mx.E4M3[1] == 2.0 ** -9 and len(plain_mx.E4M3) == 127
+    t = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(t, plain_mx.E4M3)
+
+
+@pytest.mark.parametrize("amax,e4m3,e2m1", [(448.0, 127, 133), (448.0000001, 128, 134), (1.75, 119, 125), (1.0, 119, 125), (7.0, 121, 127), (7.001, 122, 128),
+                                            (0.0, 0, 0), (2.0 ** -149, 0, 0), (math.inf, 255, 255), (3.4e38, 247, 253)])
+def test_scale_of_a_group(amax, e4m3, e2m1):
+    assert plain_mx.scale_byte(amax, 8) == e4m3 and plain_mx.scale_byte(amax, 2) == e2m1
+
+
+def test_rounding_of_the_plain_implementation():
+    """Ties go to the even code; e4m3 agrees with torch's conversion where nothing is cut off."""
+    v = np.array([0.25, 0.75, 1.25, 2.5, 3.5, 5.0, 6.9, -1.25])
+    assert plain_mx.E2M1[plain_mx.nearest(v, plain_mx.E2M1)].tolist() == [0.0, 1.0, 1.0, 2.0, 4.0, 4.0, 6.0, 1.0]
+    x = torch.randn(4096, generator=torch.Generator().manual_seed(1)) * torch.logspace(-4, 2, 4096)
+    x = x.clamp(-448, 448)
+    assert np.array_equal(plain_mx.E4M3[plain_mx.nearest(x.double().numpy(), plain_mx.E4M3)], x.abs().to(torch.float8_e4m3fn).double().numpy())
+
+
+def test_operands_on_the_host_are_refused():
+    rows = torch.zeros(2, 64)
+    with pytest.raises(KernelError):
+        mx.Mxfp4Matrix.quantize(rows)
+    with pytest.raises(KernelError):
+        mx.Mxfp4Matrix.pack(torch.zeros(2, 32, dtype=torch.uint8), torch.zeros(2, 2, dtype=torch.uint8), 64)
+    with pytest.raises(KernelError):
+        mx.Mxfp8Rows.empty(2, 64, device="cpu")
+    with pytest.raises(KernelError):
+        mx.Mxfp8Rows.pack(torch.zeros(2, 64, dtype=torch.float8_e4m3fn), torch.zeros(2, 2, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("rows,width", [(0, 64), (4, 0), (-1, 64)])
+def test_matrices_of_no_size_are_refused(rows, width):
+    with pytest.raises(KernelError):
+        mx.Mxfp4Matrix(torch.zeros(1, 1, mx.BLOCK_BYTES, dtype=torch.uint8), rows, width)
+
+
+@pytest.mark.parametrize("width,codes,scales", [(1, 128, 16), (128, 128, 16), (129, 256, 16), (512, 512, 16), (513, 640, 32), (1600, 1664, 64)])
+def test_places_of_rows(width, codes, scales):
+    """Rows of codes are whole chunks of 128, rows of scales whole pieces of 16 bytes that hold a byte for each group of the chunks."""
+    assert mx._round_up(width, mx.CHUNK) == codes and mx.Mxfp8Rows.scale_width(width) == scales and scales >= codes // 32

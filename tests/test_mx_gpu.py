@@ -1,0 +1,448 @@
+"""Products of 4-bit matrices, norms and gates with 8-bit rows, against float64."""
+
+import numpy as np
+import pytest
+import torch
+
+import plain_mx
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+@pytest.fixture(scope="module")
+def mx():
+    from liyab_amd.kernels import mx as module
+
+    return module
+
+
+def rnd(*shape, seed=0, scale=1.0, dtype=torch.float32):
+    return (scale * torch.randn(*shape, generator=torch.Generator().manual_seed(seed))).to(dtype).to(DEV)
+
+
+def matrix(mx, N, K, seed=0, scale=0.1):
+    """(the matrix, its values in float64): from plain rows made by the plain implementation, a group in eight far smaller than the others."""
+    rng = np.random.default_rng(seed)
+    w = rng.normal(size=(N, K)) * scale * np.exp2(rng.integers(-8, 1, size=(N, 1)) * (rng.random((N, 1)) < 0.125))
+    codes, scales = plain_mx.quantize(w, plain_mx.E2M1, 2)
+    m = mx.Mxfp4Matrix.pack(torch.from_numpy(plain_mx.two_a_byte(codes)).to(DEV), torch.from_numpy(scales).to(DEV), K)
+    return m, plain_mx.values(codes, scales, plain_mx.E2M1)
+
+
+def rows_of(mx, M, K, kind, seed=1):
+    """(what the product takes, its values in float64)."""
+    if kind == "mxfp8":
+        codes, scales = plain_mx.quantize(np.random.default_rng(seed).normal(size=(M, K)), plain_mx.E4M3, 8)
+        return mx.Mxfp8Rows.pack(torch.from_numpy(codes).to(DEV), torch.from_numpy(scales).to(DEV)), plain_mx.values(codes, scales, plain_mx.E4M3)
+    a = rnd(M, K, seed=seed, dtype=getattr(torch, kind))
+    return a, a.double().cpu().numpy()
+
+
+def within(got, want, bound, what):
+    got = got.double().cpu().numpy()
+    assert np.isfinite(got).all(), what
+    off = np.abs(got - want) / bound
+    assert off.max() <= 1, f"{what}: {off.max():.3g} of the bound at {np.unravel_index(off.argmax(), off.shape)}"
+
+
+def sums_bound(a, w, bias, K):
+    """Products are exact in 32 bits; every partial sum is off by at most a unit in the last place of what it can reach, in at most K / 4 + 64 steps (4 k an instruction in
+    float32, the waves' sums and the bias behind them)."""
+    return (K / 4 + 64) * 2.0 ** -23 * (np.abs(a) @ np.abs(w).T + np.abs(bias)) + 1e-30
+
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
+
+# one of everything; a strip's, a tile's and a chunk's edges, K of no whole chunk, group or piece, the sizes at which another number of rows a workgroup is taken
+SHAPES = [(1, 1, 1), (1, 16, 128), (2, 17, 40), (5, 100, 129), (15, 33, 256), (16, 64, 1600), (17, 48, 97), (31, 80, 512), (33, 40, 640), (64, 130, 2080), (65, 96, 1000),
+          (100, 257, 384), (130, 300, 576), (257, 272, 264)]
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "mxfp8"])
+@pytest.mark.parametrize("M,N,K", SHAPES)
+def test_products(mx, M, N, K, kind):
+    w, wv = matrix(mx, N, K)
+    a, av = rows_of(mx, M, K, kind)
+    bias = rnd(N, seed=2)
+    b = bias.double().cpu().numpy()
+    want, bound = av @ wv.T + b, sums_bound(av, wv, b, K)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((M, N), float("nan"), dtype=dtype, device=DEV)
+        mx.gemm_mx(a, w, bias, out=out)
+        within(out, want, bound + HALF[dtype] * (np.abs(want) + bound), f"{kind} -> {dtype}")
+    out = torch.full((M, N + 8), 3.0, device=DEV)
+    mx.gemm_mx(a, w, None, out=out[:, 4:N + 4])  # rows of a wider buffer; nothing beside them
+    within(out[:, 4:N + 4], av @ wv.T, bound + HALF[torch.float32] * (np.abs(want) + np.abs(b)), "no bias")
+    assert (out[:, :4] == 3).all() and (out[:, N + 4:] == 3).all()
+    stream = rnd(M, N, seed=3)
+    before = stream.double().cpu().numpy()
+    mx.gemm_mx(a, w, bias, residual=stream)
+    within(stream, before + want, bound + HALF[torch.float32] * (np.abs(before) + np.abs(want) + bound), "residual")
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "mxfp8"])
+@pytest.mark.parametrize("activation", ["gelu_tanh", "gelu_erf"])
+@pytest.mark.parametrize("M,N,K", [(3, 70, 96), (40, 50, 256), (150, 260, 320)])
+def test_activations(mx, M, N, K, activation, kind):
+    """The activation's slope is below 1.13; its own 32-bit evaluation: 2^-18 of the argument, whose exponential takes arguments up to 2^7 with their rounding."""
+    w, wv = matrix(mx, N, K, scale=0.3)
+    a, av = rows_of(mx, M, K, kind)
+    bias = rnd(N, seed=2)
+    b = bias.double().cpu().numpy()
+    v = av @ wv.T + b
+    want, bound = plain_mx.gelu(v, activation), 1.13 * sums_bound(av, wv, b, K) + 2.0 ** -18 * np.abs(v)
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((M, N), float("nan"), dtype=dtype, device=DEV)
+        mx.gemm_mx(a, w, bias, out=out, activation=activation)
+        within(out, want, bound + HALF[dtype] * (np.abs(want) + bound), f"{kind} -> {dtype}")
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "mxfp8"])
+@pytest.mark.parametrize("M", [1, 20, 70, 140])
+def test_rows_that_are_no_numbers_stay_by_themselves(mx, M, kind):
+    """A row of infinities or NaN makes its own results such and no other's; behind the row's end there is nothing, whatever memory holds there."""
+    N, K = 40, 200
+    w, wv = matrix(mx, N, K)
+    if kind == "mxfp8":
+        x = np.random.default_rng(5).normal(size=(M, K))
+        x[M // 2, 7] = np.inf
+        codes, scales = plain_mx.quantize(x, plain_mx.E4M3, 8)
+        a, av = mx.Mxfp8Rows.pack(torch.from_numpy(codes).to(DEV), torch.from_numpy(scales).to(DEV)), plain_mx.values(codes, scales, plain_mx.E4M3)
+    else:
+        wide = torch.full((M, K + 56), float("nan"), device=DEV, dtype=getattr(torch, kind))
+        wide[:, :K] = rnd(M, K, dtype=getattr(torch, kind))
+        wide[M // 2, 7] = float("inf")
+        a = wide[:, :K]
+        av = a.double().cpu().numpy()
+    out = torch.zeros(M, N, device=DEV)
+    mx.gemm_mx(a, w, None, out=out)
+    others = [m for m in range(M) if m != M // 2]
+    if others:
+        within(out[others], av[others] @ wv.T, sums_bound(av[others], wv, np.zeros(N), K), kind)
+    with np.errstate(invalid="ignore"):
+        want = av[M // 2] @ wv.T
+    got = out[M // 2].double().cpu().numpy()
+    assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "mxfp8"])
+def test_a_group_of_the_matrix_that_is_no_number(mx, kind):
+    codes, scales = plain_mx.quantize(np.random.default_rng(0).normal(size=(20, 96)), plain_mx.E2M1, 2)
+    scales[3, 1] = 255
+    w = mx.Mxfp4Matrix.pack(torch.from_numpy(plain_mx.two_a_byte(codes)).to(DEV), torch.from_numpy(scales).to(DEV), 96)
+    a, _ = rows_of(mx, 5, 96, kind)
+    out = torch.zeros(5, 20, device=DEV)
+    mx.gemm_mx(a, w, None, out=out)
+    nan = torch.isnan(out).cpu()
+    assert nan[:, 3].all() and not nan[:, :3].any() and not nan[:, 4:].any()
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32"])
+@pytest.mark.parametrize("shift", [0, 1, 3])
+@pytest.mark.parametrize("M,K", [(3, 128), (70, 121), (140, 264)])
+def test_rows_anywhere_in_memory(mx, M, K, shift, kind):
+    """Rows that start between pieces of 16 bytes, with strides of any number of elements."""
+    w, wv = matrix(mx, 50, K)
+    dtype = getattr(torch, kind)
+    flat = torch.full((M * (K + 5) + 16,), float("nan"), dtype=dtype, device=DEV)
+    a = flat[shift:shift + M * (K + 5)].view(M, K + 5)[:, :K]
+    a.copy_(rnd(M, K, dtype=dtype))
+    av = a.double().cpu().numpy()
+    out = torch.empty(M, 50, device=DEV)
+    mx.gemm_mx(a, w, None, out=out)
+    within(out, av @ wv.T, sums_bound(av, wv, np.zeros(50), K), kind)
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "float32", "mxfp8"])
+@pytest.mark.parametrize("M,H,Hkv,hd,K,page", [(1, 3, 3, 16, 64, 4), (33, 6, 3, 64, 128, 16), (20, 5, 1, 80, 1600, 16), (150, 4, 2, 32, 200, 48)])
+def test_products_write_pages(mx, M, H, Hkv, hd, K, page, kind):
+    """Queries to their rows, keys and values to their slots, and nothing anywhere else; a slot outside the pages is not written."""
+    q_dim, kv_dim = H * hd, Hkv * hd
+    N = q_dim + 2 * kv_dim
+    w, _ = matrix(mx, N, K)
+    a, _ = rows_of(mx, M, K, kind)
+    bias = rnd(N, seed=2)
+    dtype = torch.float32 if kind == "float32" else torch.bfloat16
+    pages = -(-M // page) + 3
+    slots = torch.randperm(pages * page, generator=torch.Generator().manual_seed(0))[:M].to(torch.int32).to(DEV)
+    if M > 1:
+        slots[1], slots[M - 1] = -1, pages * page
+    flat = torch.empty(M, N, dtype=dtype, device=DEV)
+    mx.gemm_mx(a, w, bias, out=flat)
+    kc = torch.full((pages, Hkv, page, hd), 7.0, dtype=dtype, device=DEV)
+    vc, q = kc.clone(), torch.zeros(M, q_dim, dtype=dtype, device=DEV)
+    want_k, want_v = kc.clone(), vc.clone()
+    mx.gemm_mx(a, w, bias, out=q, kv=(kc, vc, slots, q_dim))
+    for m, s in enumerate(slots.tolist()):
+        if 0 <= s < pages * page:
+            want_k[s // page, :, s % page] = flat[m, q_dim:q_dim + kv_dim].view(Hkv, hd)
+            want_v[s // page, :, s % page] = flat[m, q_dim + kv_dim:].view(Hkv, hd)
+    assert torch.equal(q, flat[:, :q_dim]) and torch.equal(kc, want_k) and torch.equal(vc, want_v)
+
+
+@pytest.mark.parametrize("M,N,K", [(40, 50, 320), (150, 264, 1000), (300, 520, 1664)])
+def test_float32_rows_have_the_same_bits_among_others(mx, M, N, K):
+    w, _ = matrix(mx, N, K)
+    a, _ = rows_of(mx, M, K, "float32")
+    out = torch.empty(M, N, device=DEV)
+    mx.gemm_mx(a, w, None, out=out)
+    for some in (slice(0, 1), slice(7, 20), slice(3, 36)):
+        part = torch.empty(some.stop - some.start, N, device=DEV)
+        mx.gemm_mx(a[some], w, None, out=part)
+        assert torch.equal(part, out[some])
+
+
+# -- the formats ------------------------------------------------------------------------------------------------------
+
+
+def hard_rows(n, d, seed=0, dtype=torch.float32):
+    """Normal values, and groups of ties, of borders, of zeros, of the least and the largest numbers, of infinities and NaN."""
+    x = torch.randn(n, d, generator=torch.Generator().manual_seed(seed)) * torch.logspace(-6, 6, n).unsqueeze(1)
+    flat = x.view(-1)
+    special = [1.75, 1.7500001, 448.0, 7.0, 7.0000005, 0.0, -0.0, 2.0 ** -149, 2.0 ** -127, 3.0e38, 1.0625, 1.1875, 0.25, -0.75, 2.5, 5.0, -6.5]
+    for i, v in enumerate(special * 3):
+        flat[(i * 37) % flat.numel()] = v
+    if d > 64 and n > 2:
+        x[1, 32:64] = 0.0
+        x[2, 40], x[0, 33] = float("inf"), float("nan")
+        x[n - 1, 32:64] = 2.0 ** -140
+    return x.to(dtype).to(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 31), (4, 96), (5, 130), (17, 264), (40, 1000)])
+def test_quantized_matrices_are_the_formats(mx, n, d, dtype):
+    x = hard_rows(n, d, dtype=dtype)
+    codes, scales = plain_mx.quantize(x.double().cpu().numpy(), plain_mx.E2M1, 2)
+    want = plain_mx.values(codes, scales, plain_mx.E2M1)
+    got = mx.Mxfp4Matrix.quantize(x)
+    packed = mx.Mxfp4Matrix.pack(torch.from_numpy(plain_mx.two_a_byte(codes)).to(DEV), torch.from_numpy(scales).to(DEV), d)
+    assert torch.equal(got.blocks, packed.blocks)
+    dense = got.dense()
+    assert np.array_equal(np.isnan(dense.cpu().numpy()), np.isnan(want))
+    fine = ~np.isnan(want) & ((np.abs(want) >= 2.0 ** -126) & (np.abs(want) < 2.0 ** 128) | (want == 0))  # (32 bits hold less below, and not 4 times 2^126)
+    assert np.array_equal(dense.double().cpu().numpy()[fine], want[fine])
+    assert torch.equal(got.dense(torch.bfloat16).float().nan_to_num(5.0)[torch.from_numpy(fine)], dense.nan_to_num(5.0)[torch.from_numpy(fine)])
+
+
+def check_rows(out, codes, scales, what):
+    """Codes and bytes of rows, and zeros behind their width."""
+    n, d = codes.shape
+    got = out.codes.cpu().numpy()
+    assert np.array_equal(got[:, :d], codes), f"{what}: {np.argwhere(got[:, :d] != codes)[:4].tolist()}"
+    assert (got[:, d:] == 0).all(), f"{what}: behind the width"
+    groups = scales.shape[1]
+    assert np.array_equal(out.scales.cpu().numpy()[:, :groups], scales), what
+    assert (out.scales.cpu().numpy()[:, groups:got.shape[1] // 32] == 0).all(), what
+
+
+def empty_rows(mx, n, d):
+    out = mx.Mxfp8Rows.empty(n, d, DEV)
+    out.codes.fill_(0xAA)
+    out.scales.fill_(0xAA)
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 31), (4, 96), (5, 130), (17, 264), (9, 2050), (3, 5001)])
+def test_rows_in_8_bits(mx, n, d, dtype):
+    x = hard_rows(n, d, dtype=dtype)
+    out = empty_rows(mx, n, d)
+    mx.rows_mx(out, x)
+    check_rows(out, *plain_mx.quantize(x.double().cpu().numpy(), plain_mx.E4M3, 8), "rows")
+    wide = torch.full((n, d + 7), float("nan"), dtype=dtype, device=DEV)
+    wide[:, 3:d + 3] = x
+    again = empty_rows(mx, n, d)
+    mx.rows_mx(again, wide[:, 3:d + 3])
+    assert torch.equal(again.codes, out.codes)
+
+
+def near_the_format(out, want, slack, what):
+    """Rows in 8 bits against the exact values before rounding, known up to `slack`: a group's byte is that of its largest magnitude give or take the slack, and every
+    number is off by half a step of its binade and the slack."""
+    n, d = want.shape
+    codes, scales = out.codes.cpu().numpy()[:, :d], out.scales.cpu().numpy()[:, : -(-d // 32)]
+    assert (out.codes.cpu().numpy()[:, d:] == 0).all(), what
+    got = plain_mx.values(codes, scales, plain_mx.E4M3)
+    for i in range(n):
+        for q in range(scales.shape[1]):
+            part = slice(32 * q, min(32 * q + 32, d))
+            mag = np.abs(want[i, part])
+            low, high = plain_mx.scale_byte(max((mag - slack[i, part]).max(), 0.0), 8), plain_mx.scale_byte((mag + slack[i, part]).max(), 8)
+            assert low <= scales[i, q] <= high, f"{what}: row {i}, group {q}: byte {scales[i, q]}, not {low} to {high}"
+            unit = 2.0 ** (int(scales[i, q]) - 127)
+            v = (mag + slack[i, part]) / unit
+            half = 2.0 ** (np.floor(np.log2(np.maximum(v, 2.0 ** -6))) - 4) * unit
+            off = np.abs(got[i, part] - want[i, part])
+            assert (off <= half * (1 + 1e-9) + slack[i, part]).all(), f"{what}: row {i}, group {q}: {off.max()} of {half.max()}"
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh", "clamped"])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 33), (5, 128), (9, 200), (2, 2500)])
+def test_gates(mx, n, d, activation):
+    gu = rnd(n, 2 * d, seed=4, scale=3.0)
+    g, u = gu.double().cpu().numpy()[:, :d], gu.double().cpu().numpy()[:, d:]
+    out = empty_rows(mx, n, d)
+    if activation == "clamped":
+        limit, slope, shift = 2.5, 1.702, 1.0
+        mx.glu_mx(out, gu, activation, clamp=(limit, slope, shift))
+        g, u = np.minimum(g, limit), np.clip(u, -limit, limit)
+        want = g / (1 + np.exp(-slope * g)) * (u + shift)
+        size = np.abs(g) * (np.abs(u) + shift)
+    else:
+        mx.glu_mx(out, gu, activation)
+        want, size = plain_mx.gelu(g, activation) * u, np.abs(g * u)
+    # an exponential whose argument (up to 2^6) is rounded, a reciprocal, three products, each of 32 bits
+    near_the_format(out, want, 2.0 ** -17 * np.maximum(np.abs(want), 2.0 ** -6 * size), activation)
+    wide = torch.full((n, 2 * d + 3), float("nan"), device=DEV)
+    wide[:, 1:2 * d + 1] = gu
+    again = empty_rows(mx, n, d)
+    mx.glu_mx(again, wide[:, 1:2 * d + 1], activation, clamp=(2.5, 1.702, 1.0) if activation == "clamped" else None)
+    assert torch.equal(again.codes, out.codes)
+
+
+@pytest.mark.parametrize("centred", [False, True])
+@pytest.mark.parametrize("added", [None, torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 40), (4, 130), (3, 512), (5, 513), (7, 1600), (2, 2049), (2, 4100), (2, 8200), (1, 20000)])
+def test_norms(mx, n, d, added, centred):
+    """Sums of d squares in 32 bits: a lane's up to 64 in a chain, then the lanes' and waves' trees: 100 roundings at most, half of them under the root; the mean likewise."""
+    x = rnd(n, d, seed=5) * torch.logspace(-2, 2, n, device=DEV).unsqueeze(1) + 0.25
+    add = None if added is None else rnd(n, d, seed=6, dtype=added)
+    w, b = 1 + 0.3 * rnd(d, seed=7), rnd(d, seed=8, scale=0.2)
+    t = x if add is None else x + add.float()
+    tv = t.double().cpu().numpy()
+    mean = tv.mean(axis=1, keepdims=True) if centred else np.zeros((n, 1))
+    r = 1 / np.sqrt(((tv - mean) ** 2).mean(axis=1, keepdims=True) + 1e-5)
+    wv, bv = w.double().cpu().numpy(), b.double().cpu().numpy()
+    slack = 100 * 2.0 ** -24 * ((np.abs(tv) + np.abs(mean) + np.abs(tv).mean(axis=1, keepdims=True) * centred) * r * np.abs(wv) + np.abs(bv) * centred) + 1e-30
+    # (a row's own deviation: what the mean's error does to the squares under the root)
+    slack *= 1 + np.abs(mean) * r
+    for out_stream in (None, torch.empty_like(x)):
+        out = empty_rows(mx, n, d)
+        mx.norm_mx(out, x, w, 1e-5, bias=b if centred else None, centred=centred, add=add, stream=out_stream)
+        near_the_format(out, (tv - mean) * r * wv + (bv if centred else 0.0), slack, f"centred {centred}")
+        if out_stream is not None:
+            assert torch.equal(out_stream, t)
+    inplace, again = x.clone(), empty_rows(mx, n, d)
+    mx.norm_mx(again, inplace, w, 1e-5, bias=b if centred else None, centred=centred, add=add, stream=inplace)
+    assert torch.equal(inplace, t) and torch.equal(again.codes, out.codes) and torch.equal(again.scales[:, : -(-d // 32)], out.scales[:, : -(-d // 32)])
+
+
+def test_norms_of_rows_that_are_no_numbers(mx):
+    """A row with an infinity has no norm; zeros have one, and their neighbours theirs."""
+    x = rnd(4, 200, seed=5)
+    x[1, 3], x[2] = float("inf"), 0.0
+    out = empty_rows(mx, 4, 200)
+    mx.norm_mx(out, x, None, 1e-5)
+    scales = out.scales.cpu().numpy()[:, :7]
+    assert scales[1, 0] == 255 and (scales[[0, 2, 3]] < 255).all() and (out.codes[2] == 0).all()
+    assert (out.codes.cpu().numpy()[:, 200:] == 0).all()
+
+
+# -- refusals -----------------------------------------------------------------------------------------------------------
+
+
+def test_refusals(mx):
+    from liyab_amd.errors import KernelError
+
+    w, _ = matrix(mx, 32, 64)
+    a, out = rnd(4, 64, dtype=torch.bfloat16), torch.empty(4, 32, device=DEV)
+    rows = mx.Mxfp8Rows.empty(4, 64)
+    bad = [
+        lambda: mx.gemm_mx(rnd(4, 65, dtype=torch.bfloat16), w, None, out=out),
+        lambda: mx.gemm_mx(a.half(), w, None, out=out),
+        lambda: mx.gemm_mx(a.cpu(), w, None, out=out),
+        lambda: mx.gemm_mx(a.t(), w, None, out=out),
+        lambda: mx.gemm_mx(a, w, None, out=out[:3]),
+        lambda: mx.gemm_mx(a, w, None),
+        lambda: mx.gemm_mx(a, w, rnd(31), out=out),
+        lambda: mx.gemm_mx(a, w, None, residual=out.bfloat16()),
+        lambda: mx.gemm_mx(mx.Mxfp8Rows.empty(4, 96), w, None, out=out),
+        lambda: mx.rows_mx(rows, rnd(4, 65)),
+        lambda: mx.rows_mx(rows, rnd(3, 64)),
+        lambda: mx.rows_mx(rows, rnd(4, 64).half()),
+        lambda: mx.glu_mx(rows, rnd(4, 64), "silu"),
+        lambda: mx.glu_mx(rows, rnd(4, 128), "relu"),
+        lambda: mx.glu_mx(rows, rnd(4, 128), "clamped"),
+        lambda: mx.glu_mx(rows, rnd(4, 128), "clamped", clamp=(0.0, 1.0, 0.0)),
+        lambda: mx.glu_mx(rows, rnd(4, 128, dtype=torch.bfloat16), "silu"),
+        lambda: mx.norm_mx(rows, rnd(4, 64, dtype=torch.bfloat16), None, 1e-5),
+        lambda: mx.norm_mx(rows, rnd(4, 128)[:, :64], None, 1e-5),
+        lambda: mx.norm_mx(rows, rnd(4, 64), rnd(63), 1e-5),
+        lambda: mx.norm_mx(rows, rnd(4, 64), None, 1e-5, add=rnd(3, 64)),
+        lambda: mx.norm_mx(rows, rnd(4, 64), None, 1e-5, stream=rnd(4, 64, dtype=torch.bfloat16)),
+        lambda: mx.norm_mx(mx.Mxfp8Rows.empty(1, 65537), rnd(1, 65537), None, 1e-5),
+        lambda: mx.Mxfp4Matrix.quantize(rnd(4, 64).half()),
+        lambda: mx.Mxfp4Matrix.pack(torch.zeros(4, 32, dtype=torch.uint8, device=DEV), torch.zeros(4, 3, dtype=torch.uint8, device=DEV), 64),
+        lambda: mx.Mxfp4Matrix(w.blocks, 32, 200),
+        lambda: mx.Mxfp4Matrix(w.blocks.view(-1)[1:1 + 2 * 1088].view(2, 1, 1088), 32, 64) if w.blocks.numel() > 2 * 1088 else mx.Mxfp4Matrix(w.blocks, 33, 64),
+        lambda: mx.Mxfp8Rows(rows.codes[:, :64], rows.scales, 64),
+        lambda: mx.Mxfp8Rows(rows.codes, rows.scales[:2], 64),
+        lambda: mx.Mxfp8Rows.pack(torch.zeros(4, 64, device=DEV), torch.zeros(4, 2, dtype=torch.uint8, device=DEV)),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(KernelError):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+def test_no_rows(mx):
+    w, _ = matrix(mx, 32, 64)
+    mx.gemm_mx(torch.empty(0, 64, dtype=torch.bfloat16, device=DEV), w, None, out=torch.empty(0, 32, device=DEV))
+    none = mx.Mxfp8Rows.empty(0, 64)
+    mx.rows_mx(none, torch.empty(0, 64, device=DEV))
+    mx.glu_mx(none, torch.empty(0, 128, device=DEV), "silu")
+    mx.norm_mx(none, torch.empty(0, 64, device=DEV), None, 1e-5)
+    mx.gemm_mx(none, w, None, out=torch.empty(0, 32, device=DEV))
+
+
+# -- together -------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("n", [1, 9, 150])
+def test_a_gated_feed_forward_in_a_graph_and_on_another_stream(mx, n):
+    """norm -> [gate | up] -> gate -> down, added to the stream: eager, on a stream of its own, and replayed from a graph with new rows, the same bits each time; the last
+    product against float64 of the rows that it read."""
+    d, ff = 192, 328
+    w1, _ = matrix(mx, 2 * ff, d, seed=1)
+    w2, w2v = matrix(mx, d, ff, seed=2)
+    nw = 1 + 0.2 * rnd(d, seed=3)
+    x, y = torch.empty(n, d, device=DEV), torch.empty(n, d, device=DEV)
+    h, inner, gu = mx.Mxfp8Rows.empty(n, d), mx.Mxfp8Rows.empty(n, ff), torch.empty(n, 2 * ff, device=DEV)
+
+    def run():
+        mx.norm_mx(h, x, nw, 1e-5, add=y, stream=x)
+        mx.gemm_mx(h, w1, None, out=gu)
+        mx.glu_mx(inner, gu, "silu")
+        mx.gemm_mx(inner, w2, None, residual=x)
+
+    def fill(seed):
+        x.copy_(rnd(n, d, seed=seed))
+        y.copy_(rnd(n, d, seed=seed + 1))
+
+    def eager(seed):
+        fill(seed)
+        run()
+        torch.cuda.synchronize()
+        return x.clone()
+
+    want = [eager(10), eager(20)]
+    rows = plain_mx.values(inner.codes.cpu().numpy()[:, :ff], inner.scales.cpu().numpy()[:, : -(-ff // 32)], plain_mx.E4M3)
+    before = (rnd(n, d, seed=20) + rnd(n, d, seed=21)).double().cpu().numpy()
+    within(want[1], before + rows @ w2v.T, sums_bound(rows, w2v, np.zeros(d), ff) + 2.0 ** -23 * (np.abs(before) + np.abs(rows @ w2v.T)), "down")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        fill(10)
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(x, want[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    for seed, expected in ((10, want[0]), (20, want[1]), (10, want[0])):
+        fill(seed)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(x, expected)
