@@ -238,5 +238,5 @@ int liyab_mx_glu(void* codes, int64_t ldo, void* scales, int64_t lds, const floa
 int liyab_mx_norm(void* codes, int64_t ldo, void* scales, int64_t lds, const float* x, const void* add, int add_dtype, float* stream_out,
                   const float* weight, const float* bias, float eps, int centred, int n, int d, hipStream_t stream);
 int liyab_mx_product(const void* a, int64_t lda, const void* a_scales, int64_t lds, int rows, const void* blocks, int M, int N, int K,
-                     const liyab::EpiParams* epi, hipStream_t stream);
+                     int tile, const liyab::EpiParams* epi, hipStream_t stream);
 }  // extern "C"

@@ -14,23 +14,11 @@
 #include "epilogue.h"
 #include "launchers.h"
 #include "mx.h"
+#include "mx_product.h"
 
 namespace liyab {
 
 typedef __attribute__((ext_vector_type(4))) float mx_f32x4;
-typedef __attribute__((ext_vector_type(8))) __bf16 mx_bf16x8;
-
-enum : int { kRowsBF16 = 0, kRowsF32 = 1, kRowsMx = 2 };
-
-struct MxRowsIn {
-    const void* a;          // [M, lda], bfloat16, float32 or codes
-    int64_t lda;            // elements
-    const uint8_t* scales;  // [M, lds] of rows in 8 bits
-    int64_t lds;
-};
-
-// What a load behind a row's end reads instead: zeros, so that the zeros of the matrix there meet numbers.
-__device__ __constant__ const uint32_t mx_zeros[4] = {0, 0, 0, 0};
 
 // A chunk of one row as the matrix instructions take it.
 template <int ROWS>
@@ -72,16 +60,10 @@ __device__ __forceinline__ void load_row(MxRowPart<ROWS>& part, const uint8_t* r
 #pragma unroll
         for (int j = 0; j < kMxGroup / PER; ++j) {
             const uint8_t* p = row + static_cast<int64_t>(k + j * PER) * SIZE;
-            if (TAIL && k + j * PER >= K) p = reinterpret_cast<const uint8_t*>(mx_zeros);
+            if (TAIL && k + j * PER >= K) p = reinterpret_cast<const uint8_t*>(mx_zeros());
             part.piece[j] = *reinterpret_cast<const uint4*>(p);
         }
     }
-}
-
-__device__ __forceinline__ mx_bf16x8 eight_of(uint32_t word, float power) {
-    const mx_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 1),
-                    c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 2), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(word, power, 3);
-    return mx_bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
 // acc[i] += matrix rows 4 g + i of the block times the lane's row.
@@ -92,7 +74,7 @@ __device__ __forceinline__ void multiply_block(mx_f32x4 (&acc)[MT], const uint4&
         const float power = mx_power(scale);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const mx_bf16x8 w = eight_of(word[j], power);
+            const mx_bf16x8 w = mx_eight_of(word[j], power);
 #pragma unroll
             for (int t = 0; t < MT; ++t) acc[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, rows[t].eight(j), acc[t], 0, 0, 0);
         }
@@ -201,7 +183,8 @@ static int launch_product(const MxRowsIn& in, const uint8_t* blocks, int M, int 
 }
 
 template <int ROWS>
-static int product_of_rows(const MxRowsIn& in, const uint8_t* blocks, int M, int N, int K, const EpiParams& epi, hipStream_t stream) {
+static int product_of_rows(int tile, const MxRowsIn& in, const uint8_t* blocks, int M, int N, int K, const EpiParams& epi, hipStream_t stream) {
+    if (tile >= 0 && (M > 64 || tile > 0) && ROWS != kRowsF32) return launch_mx_tiles(ROWS, tile, in, blocks, M, N, K, epi, stream);
     if (M <= 16) return launch_product<ROWS, 1, 1, 2, 8>(in, blocks, M, N, K, epi, stream);
     if (M <= 32) return launch_product<ROWS, 2, 1, 1, 8>(in, blocks, M, N, K, epi, stream);
     return launch_product<ROWS, 4, 1, 1, 8>(in, blocks, M, N, K, epi, stream);
@@ -212,8 +195,10 @@ static int product_of_rows(const MxRowsIn& in, const uint8_t* blocks, int M, int
 using namespace liyab;
 
 // a: rows [M, lda] of `rows` 0: bfloat16, 1: float32, 2: e4m3 codes (padded with zeros to whole chunks) with their scales [M, lds].
-extern "C" int liyab_mx_product(const void* a, int64_t lda, const void* a_scales, int64_t lds, int rows, const void* blocks, int M, int N, int K, const EpiParams* epi,
-                                hipStream_t stream) {
+// tile: 0 chooses the kernel from the sizes, -1 takes this file's whatever they are (one order of every sum, so that a row's bits follow K alone), a positive
+// number a tile of mx_tiles.hip.
+extern "C" int liyab_mx_product(const void* a, int64_t lda, const void* a_scales, int64_t lds, int rows, const void* blocks, int M, int N, int K, int tile,
+                                const EpiParams* epi, hipStream_t stream) {
     LIYAB_REQUIRE(a && blocks && epi, "mx_product: null pointer");
     LIYAB_REQUIRE(M >= 0 && N > 0 && K > 0, "mx_product: bad sizes");
     if (M == 0) return 0;
@@ -225,10 +210,10 @@ extern "C" int liyab_mx_product(const void* a, int64_t lda, const void* a_scales
     if (rows == kRowsMx) {
         LIYAB_REQUIRE(a_scales && lda >= static_cast<int64_t>(mx_chunks(K)) * kMxChunk && lda % 16 == 0 && lds >= mx_chunks(K) * 4, "mx_product: rows in 8 bits are padded to %d codes",
                       mx_chunks(K) * kMxChunk);
-        return product_of_rows<kRowsMx>(in, b, M, N, K, *epi, stream);
+        return product_of_rows<kRowsMx>(tile, in, b, M, N, K, *epi, stream);
     }
     const int per = rows == kRowsBF16 ? 8 : 4;
     LIYAB_REQUIRE(rows == kRowsBF16 || rows == kRowsF32, "mx_product: unknown kind of rows %d", rows);
     LIYAB_REQUIRE(K % per == 0 && lda % per == 0 && lda >= K, "mx_product: rows of whole pieces of 16 bytes are taken (K = %d, row stride %lld)", K, static_cast<long long>(lda));
-    return rows == kRowsBF16 ? product_of_rows<kRowsBF16>(in, b, M, N, K, *epi, stream) : product_of_rows<kRowsF32>(in, b, M, N, K, *epi, stream);
+    return rows == kRowsBF16 ? product_of_rows<kRowsBF16>(tile, in, b, M, N, K, *epi, stream) : product_of_rows<kRowsF32>(tile, in, b, M, N, K, *epi, stream);
 }

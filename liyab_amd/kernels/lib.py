@@ -156,7 +156,7 @@ _SIGNATURES = {
     "liyab_mx_glu": [P, c_int64, P, c_int64, P, c_int64, c_int, c_int, c_int, c_float, c_float, c_float, P],
     "liyab_mx_norm": [P, c_int64, P, c_int64, P, P, c_int, P, P, P, c_float, c_int, c_int, c_int, P],
     "liyab_mx_align": [P, c_int, P, c_int64, c_int, c_int, c_int, P],
-    "liyab_mx_product": [P, c_int64, P, c_int64, c_int, P, c_int, c_int, c_int, _EPI_PTR, P],
+    "liyab_mx_product": [P, c_int64, P, c_int64, c_int, P, c_int, c_int, c_int, c_int, _EPI_PTR, P],
 }
 
 

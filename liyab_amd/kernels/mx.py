@@ -233,7 +233,7 @@ def norm_mx(out: Mxfp8Rows, x: torch.Tensor, weight: Optional[torch.Tensor], eps
 
 
 def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-            activation: str = "none", kv=None) -> None:
+            activation: str = "none", kv=None, tile: int = 0) -> None:
     """out = act(a . w^T + bias), or residual += a . w^T + bias, or the paged query, key and value product (`kv` as `ops.gemm` takes it). a [M, K]: bfloat16 or
     float32 with contiguous rows, or `Mxfp8Rows`; out [M, N] bfloat16 or float32, residual float32. Products are exact in 32 bits
     and their sums are 32-bit. float32 rows: every sum is a chain of 32-bit multiply-adds in an order that does not follow M."""
@@ -269,7 +269,7 @@ def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[to
         ptr, lda = a.data_ptr(), K
     elif kind == _ROWS_MX:
         K = w.width
-    _lib.call("liyab_mx_product", ptr, lda, scales, lds, kind, w.blocks.data_ptr(), M, w.rows, K, ctypes.byref(e), _stream())
+    _lib.call("liyab_mx_product", ptr, lda, scales, lds, kind, w.blocks.data_ptr(), M, w.rows, K, tile, ctypes.byref(e), _stream())
 
 
 class _Like:

@@ -46,10 +46,11 @@ def within(got, want, bound, what):
     assert off.max() <= 1, f"{what}: {off.max():.3g} of the bound at {np.unravel_index(off.argmax(), off.shape)}"
 
 
-def sums_bound(a, w, bias, K):
+def sums_bound(a, w, bias, K, cut=False):
     """Products are exact in 32 bits; every partial sum is off by at most a unit in the last place of what it can reach, in at most K / 4 + 64 steps (4 k an instruction in
-    float32, the waves' sums and the bias behind them)."""
-    return (K / 4 + 64) * 2.0 ** -23 * (np.abs(a) @ np.abs(w).T + np.abs(bias)) + 1e-30
+    float32, the waves' sums and the bias behind them). `cut`: the scaled matrix instruction (8-bit rows, more than 64 of them) adds eight neighbouring products without what lies
+    below 2^-13 of the largest: each is off by less than that, eight of them by 2^-10 of the largest, which their sizes' sum is no less than."""
+    return (2.0 ** -10 * cut + (K / 4 + 64) * 2.0 ** -23) * (np.abs(a) @ np.abs(w).T + np.abs(bias)) + 1e-30
 
 
 HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -24}
@@ -66,7 +67,8 @@ def test_products(mx, M, N, K, kind):
     a, av = rows_of(mx, M, K, kind)
     bias = rnd(N, seed=2)
     b = bias.double().cpu().numpy()
-    want, bound = av @ wv.T + b, sums_bound(av, wv, b, K)
+    cut = kind == "mxfp8" and M > 64
+    want, bound = av @ wv.T + b, sums_bound(av, wv, b, K, cut)
     for dtype in (torch.float32, torch.bfloat16):
         out = torch.full((M, N), float("nan"), dtype=dtype, device=DEV)
         mx.gemm_mx(a, w, bias, out=out)
@@ -91,11 +93,40 @@ def test_activations(mx, M, N, K, activation, kind):
     bias = rnd(N, seed=2)
     b = bias.double().cpu().numpy()
     v = av @ wv.T + b
-    want, bound = plain_mx.gelu(v, activation), 1.13 * sums_bound(av, wv, b, K) + 2.0 ** -18 * np.abs(v)
+    want, bound = plain_mx.gelu(v, activation), 1.13 * sums_bound(av, wv, b, K, kind == "mxfp8" and M > 64) + 2.0 ** -18 * np.abs(v)
     for dtype in (torch.float32, torch.bfloat16):
         out = torch.full((M, N), float("nan"), dtype=dtype, device=DEV)
         mx.gemm_mx(a, w, bias, out=out, activation=activation)
         within(out, want, bound + HALF[dtype] * (np.abs(want) + bound), f"{kind} -> {dtype}")
+
+
+@pytest.mark.parametrize("kind", ["bfloat16", "mxfp8"])
+@pytest.mark.parametrize("tile", [1, 2])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 8), (64, 64, 128), (129, 100, 136), (128, 128, 256), (257, 300, 1000), (300, 257, 384), (512, 520, 264)])
+def test_tiles(mx, M, N, K, tile, kind):
+    """Every tile at sizes inside it and past its edges, every epilogue. In the 2-norm what the scaled instruction cuts off stays below 1e-4: products have six
+    significant bits, so only those under 2^-7 of their eight's largest lose any, a tenth of them at most, 2^-13 of it and a third of that in the mean."""
+    w, wv = matrix(mx, N, K)
+    a, av = rows_of(mx, M, K, kind)
+    bias = rnd(N, seed=2)
+    b = bias.double().cpu().numpy()
+    want, bound = av @ wv.T + b, sums_bound(av, wv, b, K, kind == "mxfp8")
+    for dtype in (torch.float32, torch.bfloat16):
+        out = torch.full((M + 3, N), float("nan"), dtype=dtype, device=DEV)
+        mx.gemm_mx(a, w, bias, out=out[:M], tile=tile)
+        within(out[:M], want, bound + HALF[dtype] * (np.abs(want) + bound), f"{kind} -> {dtype}")
+        assert torch.isnan(out[M:]).all()
+        if dtype == torch.float32:
+            off = np.linalg.norm(out[:M].double().cpu().numpy() - want) / max(np.linalg.norm(av @ wv.T), 1e-30)
+            assert off < (1e-4 if kind == "mxfp8" else 1e-6), off
+        act = torch.full((M, N), float("nan"), dtype=dtype, device=DEV)
+        mx.gemm_mx(a, w, bias, out=act, activation="gelu_erf", tile=tile)
+        exact = plain_mx.gelu(want, "gelu_erf")
+        within(act, exact, 1.13 * bound + 2.0 ** -18 * np.abs(want) + HALF[dtype] * (np.abs(exact) + bound), "gelu_erf")
+    stream = rnd(M, N, seed=3)
+    before = stream.double().cpu().numpy()
+    mx.gemm_mx(a, w, bias, residual=stream, tile=tile)
+    within(stream, before + want, bound + HALF[torch.float32] * (np.abs(before) + np.abs(want) + bound), "residual")
 
 
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "mxfp8"])
@@ -119,7 +150,7 @@ def test_rows_that_are_no_numbers_stay_by_themselves(mx, M, kind):
     mx.gemm_mx(a, w, None, out=out)
     others = [m for m in range(M) if m != M // 2]
     if others:
-        within(out[others], av[others] @ wv.T, sums_bound(av[others], wv, np.zeros(N), K), kind)
+        within(out[others], av[others] @ wv.T, sums_bound(av[others], wv, np.zeros(N), K, kind == "mxfp8" and M > 64), kind)
     with np.errstate(invalid="ignore"):
         want = av[M // 2] @ wv.T
     got = out[M // 2].double().cpu().numpy()
@@ -430,7 +461,7 @@ def test_a_gated_feed_forward_in_a_graph_and_on_another_stream(mx, n):
     want = [eager(10), eager(20)]
     rows = plain_mx.values(inner.codes.cpu().numpy()[:, :ff], inner.scales.cpu().numpy()[:, : -(-ff // 32)], plain_mx.E4M3)
     before = (rnd(n, d, seed=20) + rnd(n, d, seed=21)).double().cpu().numpy()
-    within(want[1], before + rows @ w2v.T, sums_bound(rows, w2v, np.zeros(d), ff) + 2.0 ** -23 * (np.abs(before) + np.abs(rows @ w2v.T)), "down")
+    within(want[1], before + rows @ w2v.T, sums_bound(rows, w2v, np.zeros(d), ff, n > 64) + 2.0 ** -23 * (np.abs(before) + np.abs(rows @ w2v.T)), "down")
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
