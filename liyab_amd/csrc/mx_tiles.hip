@@ -180,15 +180,10 @@ static int tile_of_epilogue(const MxRowsIn& in, const uint8_t* blocks, int M, in
 #undef LIYAB_TILE
 }
 
-template <int ROWS>
-static int tile_of_size(int tile, const MxRowsIn& in, const uint8_t* blocks, int M, int N, int K, const EpiParams& epi, hipStream_t stream) {
-    if (tile == 1) return tile_of_epilogue<ROWS, 2, 2, 4, 4>(in, blocks, M, N, K, epi, stream);
-    return tile_of_epilogue<ROWS, 2, 4, 8, 4>(in, blocks, M, N, K, epi, stream);
-}
-
 int launch_mx_tiles(int kind, int tile, const MxRowsIn& in, const uint8_t* blocks, int M, int N, int K, const EpiParams& epi, hipStream_t stream) {
-    if (tile == 0) tile = static_cast<int64_t>((M + 255) / 256) * ((N + 255) / 256) >= 256 ? 2 : 1;
-    return kind == kRowsMx ? tile_of_size<kRowsMx>(tile, in, blocks, M, N, K, epi, stream) : tile_of_size<kRowsBF16>(tile, in, blocks, M, N, K, epi, stream);
+    if (kind == kRowsMx)
+        return tile == kMxTile128 ? tile_of_epilogue<kRowsMx, 2, 2, 4, 4>(in, blocks, M, N, K, epi, stream) : tile_of_epilogue<kRowsMx, 2, 4, 8, 4>(in, blocks, M, N, K, epi, stream);
+    return tile == kMxTile128 ? tile_of_epilogue<kRowsBF16, 2, 2, 4, 4>(in, blocks, M, N, K, epi, stream) : tile_of_epilogue<kRowsBF16, 2, 4, 8, 4>(in, blocks, M, N, K, epi, stream);
 }
 
 }  // namespace liyab

@@ -24,7 +24,8 @@ import torch
 
 from ..errors import KernelError
 from . import lib as _lib
-from .ops import (ACTIVATION_EPILOGUE, BF16, EPI_QKV_PAGED, EPI_RESIDUAL, F32, GLU_ACTIVATIONS, _dev, _epilogue, _f32vec, _ptr, _rows, _stream, dtype_code)
+from . import ops
+from .ops import ACTIVATION_EPILOGUE, EPI_QKV_PAGED, EPI_RESIDUAL, F32, GLU_ACTIVATIONS, _dev, _epilogue, _f32vec, _ptr, _rows, _stream, dtype_code
 
 GROUP = 32
 CHUNK = 128  # k of a block of a matrix; rows of codes are padded to whole chunks
@@ -63,7 +64,7 @@ class Mxfp4Matrix:
         _dev(blocks, "blocks")
         if blocks.dtype != torch.uint8 or tuple(blocks.shape) != shape or not blocks.is_contiguous() or blocks.data_ptr() % 16:
             raise KernelError(f"a 4-bit matrix of {rows} x {width} needs contiguous uint8 blocks {shape} on a 16-byte boundary, got {tuple(blocks.shape)} {blocks.dtype}")
-        self.blocks, self.rows, self.width = blocks, rows, width
+        self.blocks, self.rows, self.width, self.index = blocks, rows, width, blocks.get_device()
 
     @property
     def shape(self):
@@ -126,6 +127,7 @@ class Mxfp8Rows:
         _dev(codes, "codes")
         if codes.data_ptr() % 16:
             raise KernelError("codes must start on a 16-byte boundary")
+        self.index = codes.get_device()
 
     @staticmethod
     def scale_width(width: int) -> int:
@@ -163,24 +165,37 @@ def _check_out(out: Mxfp8Rows, n: int, d: int, what: str) -> None:
         raise KernelError(f"{what}: the rows have places for [{out.n}, {out.width}], not [{n}, {d}]")
 
 
-def _same_device(what: str, device, *tensors) -> None:
-    """Every operand lies on the device that launches go to."""
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"{what}: operands on {device}, the current device is cuda:{torch.cuda.current_device()}")
+def _stream_on(index: int) -> int:
+    """The stream that launches go to (`ops._stream`; asked for without the objects that torch makes around it, 2 us of a call)."""
+    return ops._pinned_stream if ops._pinned_stream is not None else torch._C._cuda_getCurrentRawStream(index)
+
+
+def _refuse_devices(what: str, index: int, *tensors) -> None:
+    """Every operand lies on the device that launches go to; `_on` has found one that does not."""
     for t in tensors:
-        if t is not None and t.device != device:
-            raise KernelError(f"{what}: operands on {device} and {t.device}")
+        if t is not None and t.get_device() != index:
+            raise KernelError(f"{what}: operands on {t.device} and cuda:{index}")
+    raise KernelError(f"{what}: operands on cuda:{index}, the current device is cuda:{torch.cuda.current_device()}")
+
+
+def _on(what: str, index: int, *tensors) -> int:
+    if index != torch._C._cuda_getDevice():
+        _refuse_devices(what, index)
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            _refuse_devices(what, index, t)
+    return _stream_on(index)
 
 
 def rows_mx(out: Mxfp8Rows, x: torch.Tensor) -> None:
     """out = x [n, d] (float32 or bfloat16, rows contiguous) in 8 bits."""
     ldx = _rows(x, "x")
     _check_out(out, x.shape[0], x.shape[1], "rows_mx")
-    _same_device("rows_mx", out.device, x)
+    stream = _on("rows_mx", out.index, x)
     if out.n == 0:
         return
     _lib.call("liyab_mx_rows", out.codes.data_ptr(), out.codes.shape[1], out.scales.data_ptr(), out.scales.shape[1], x.data_ptr(), dtype_code(x.dtype), ldx,
-              x.shape[0], x.shape[1], _stream())
+              out.n, out.width, stream)
 
 
 def glu_mx(out: Mxfp8Rows, gu: torch.Tensor, activation: str, clamp=None) -> None:
@@ -191,7 +206,7 @@ def glu_mx(out: Mxfp8Rows, gu: torch.Tensor, activation: str, clamp=None) -> Non
     if gu.dtype != torch.float32 or d2 != 2 * out.width:
         raise KernelError(f"glu_mx: needs float32 [n, {2 * out.width}], got {tuple(gu.shape)} {gu.dtype}")
     _check_out(out, n, d2 // 2, "glu_mx")
-    _same_device("glu_mx", out.device, gu)
+    stream = _on("glu_mx", out.index, gu)
     if (activation == "clamped") != (clamp is not None) or (clamp is None and activation not in GLU_ACTIVATIONS):
         raise KernelError(f"glu_mx: activation '{activation}' with clamp {clamp}")
     limit, slope, shift = clamp or (1.0, 1.0, 0.0)
@@ -201,7 +216,7 @@ def glu_mx(out: Mxfp8Rows, gu: torch.Tensor, activation: str, clamp=None) -> Non
         return
     act = CLAMPED_GLU if clamp is not None else GLU_ACTIVATIONS[activation]
     _lib.call("liyab_mx_glu", out.codes.data_ptr(), out.codes.shape[1], out.scales.data_ptr(), out.scales.shape[1], gu.data_ptr(), ld, n, d2 // 2, act,
-              float(limit), float(slope), float(shift), _stream())
+              float(limit), float(slope), float(shift), stream)
 
 
 def norm_mx(out: Mxfp8Rows, x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, *, bias: Optional[torch.Tensor] = None, centred: bool = False,
@@ -225,51 +240,57 @@ def norm_mx(out: Mxfp8Rows, x: torch.Tensor, weight: Optional[torch.Tensor], eps
             raise KernelError(f"norm_mx: what is added must be contiguous [{n}, {d}], got {tuple(add.shape)}")
     if stream is not None and (stream.dtype != torch.float32 or stream.shape != x.shape or not stream.is_contiguous()):
         raise KernelError(f"norm_mx: the stream must be contiguous float32 [{n}, {d}], got {tuple(stream.shape)} {stream.dtype}")
-    _same_device("norm_mx", out.device, x, weight, bias, add, stream)
+    to = _on("norm_mx", out.index, x, weight, bias, add, stream)
     if n == 0:
         return
     _lib.call("liyab_mx_norm", out.codes.data_ptr(), out.codes.shape[1], out.scales.data_ptr(), out.scales.shape[1], x.data_ptr(), _ptr(add), code, _ptr(stream),
-              _ptr(weight), _ptr(bias), float(eps), 1 if centred else 0, n, d, _stream())
+              _ptr(weight), _ptr(bias), float(eps), 1 if centred else 0, n, d, to)
 
 
 def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
-            activation: str = "none", kv=None, tile: int = 0) -> None:
+            activation: str = "none", kv=None, shape: int = 0) -> None:
     """out = act(a . w^T + bias), or residual += a . w^T + bias, or the paged query, key and value product (`kv` as `ops.gemm` takes it). a [M, K]: bfloat16 or
     float32 with contiguous rows, or `Mxfp8Rows`; out [M, N] bfloat16 or float32, residual float32. Products are exact in 32 bits
-    and their sums are 32-bit. float32 rows: every sum is a chain of 32-bit multiply-adds in an order that does not follow M."""
+    and their sums are 32-bit; where 8-bit rows are many, eight neighbouring products are added to 14 bits below their largest first (csrc/mx_tiles.hip). A row has the same
+    bits whatever the other rows if it is float32, or under `ops.batch_invariant`. `shape`: the workgroups' (csrc/mx_product.hip; 0: chosen from the sizes)."""
+    index, K, N = w.index, w.width, w.rows
+    if type(a) is Mxfp8Rows:
+        kind, operand, M, dtype = _ROWS_MX, a.codes, a.n, torch.bfloat16
+        if a.width != K:
+            raise KernelError(f"gemm_mx: rows of {a.width} values, a matrix of width {K}")
+        lda, scales, lds = operand.shape[1], a.scales.data_ptr(), a.scales.shape[1]
+    else:
+        lda, operand, scales, lds, dtype = _rows(a, "a"), a, None, 0, a.dtype
+        M, width = a.shape
+        if width != K or (dtype is not torch.bfloat16 and dtype is not torch.float32):
+            raise KernelError(f"gemm_mx: a {tuple(a.shape)} {dtype} does not fit a matrix of {N} x {K}")
+        kind, per = (_ROWS_BF16, 8) if dtype is torch.bfloat16 else (_ROWS_F32, 4)
+    stream = _on("gemm_mx", index, operand, bias, out, residual, *(kv[:3] if kv is not None else ()))
     if kv is not None:
-        epilogue = EPI_QKV_PAGED
-    elif residual is not None:
-        epilogue = EPI_RESIDUAL
+        e = _epilogue(_Like(M, dtype), w, bias, out, None, EPI_QKV_PAGED, kv)
     else:
-        epilogue = ACTIVATION_EPILOGUE[activation]
-    if isinstance(a, Mxfp8Rows):
-        if a.width != w.width:
-            raise KernelError(f"gemm_mx: rows of {a.width} values, a matrix of width {w.width}")
-        kind, ptr, lda, scales, lds, M = _ROWS_MX, a.codes.data_ptr(), a.codes.shape[1], a.scales.data_ptr(), a.scales.shape[1], a.n
-        rows = _Like(M, torch.bfloat16)
-    else:
-        lda = _rows(a, "a")
-        M, K = a.shape
-        if K != w.width or a.dtype not in (torch.bfloat16, torch.float32):
-            raise KernelError(f"gemm_mx: a {tuple(a.shape)} {a.dtype} does not fit a matrix of {w.rows} x {w.width}")
-        kind, per = (_ROWS_BF16, 8) if a.dtype == torch.bfloat16 else (_ROWS_F32, 4)
-        ptr, scales, lds, rows = a.data_ptr(), None, 0, a
-    _same_device("gemm_mx", w.blocks.device, a, bias, out, residual, *(kv[:3] if kv is not None else ()))
-    e = _epilogue(rows, w, bias, out, residual, epilogue, kv)
+        _f32vec(bias, "bias", N)
+        if residual is not None:
+            if residual.dtype is not torch.float32 or residual.shape != (M, N):
+                raise KernelError("gemm_mx: needs a float32 residual [M, N]")
+            e = _lib.EpiParams(EPI_RESIDUAL, F32, _ptr(bias), None, 0, residual.data_ptr(), _rows(residual, "residual"))
+        else:
+            if out is None or out.shape != (M, N):
+                raise KernelError("gemm_mx: out must be [M, N]")
+            e = _lib.EpiParams(ACTIVATION_EPILOGUE[activation], dtype_code(out.dtype), _ptr(bias), out.data_ptr(), _rows(out, "out"))
+        e.exact = 1 if kind == _ROWS_F32 else 0
     if M == 0:
         return
+    ptr = operand.data_ptr()
     if kind != _ROWS_MX and (K % per or lda % per or ptr % 16):
         # rows that are no whole pieces of 16 bytes, or lie between them: a copy that is, in memory that only this call has (a list of launches
         # that is run again would find somebody else's there)
         _lib.not_recordable()
-        K = _round_up(K, per)
-        a = torch.empty((M, K), dtype=a.dtype, device=a.device)
-        _lib.call("liyab_mx_align", a.data_ptr(), K, ptr, lda, a.element_size(), M, w.width, _stream())
-        ptr, lda = a.data_ptr(), K
-    elif kind == _ROWS_MX:
-        K = w.width
-    _lib.call("liyab_mx_product", ptr, lda, scales, lds, kind, w.blocks.data_ptr(), M, w.rows, K, tile, ctypes.byref(e), _stream())
+        K = lda = _round_up(K, per)
+        own = torch.empty((M, K), dtype=dtype, device=a.device)
+        _lib.call("liyab_mx_align", own.data_ptr(), K, ptr, _rows(a, "a"), a.element_size(), M, w.width, stream)
+        ptr = own.data_ptr()
+    _lib.call("liyab_mx_product", ptr, lda, scales, lds, kind, w.blocks.data_ptr(), M, N, K, shape or (-1 if ops._invariant else 0), ctypes.byref(e), stream)
 
 
 class _Like:
