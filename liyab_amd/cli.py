@@ -41,6 +41,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--ctx", type=int, default=None, help="context length (default: the model's)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"],
                     help="precision of the whole path (default bfloat16)")
+    ap.add_argument("--weights", default=None, choices=["mxfp4"], help="matrices of attention's and the feed-forwards' products in 4 bits, rounded at load (default: as --dtype says)")
+    ap.add_argument("--rows", default=None, choices=["mxfp8"], help="with --weights: these products take their rows in 8 bits (default: as --dtype says)")
     ap.add_argument("--json", action="store_true", help="stdout: one JSON line after loading and one for the generation")
     ap.add_argument("--tokenize", action="store_true", help="print the prompt's token ids and exit")
     ap.add_argument("--phases", action="store_true",
@@ -98,7 +100,7 @@ def main(argv=None) -> int:
         engine = Engine(model_dir, dtype=args.dtype, device=args.device, page_size=args.page_size,
                         num_pages=args.num_pages, max_num_seqs=args.max_num_seqs,
                         max_batched_tokens=args.max_batched_tokens, prefill_chunk=args.prefill_chunk, ctx=args.ctx,
-                        phases=args.phases)
+                        phases=args.phases, weights=args.weights, rows=args.rows)
         engine.warmup()  # kernels' code loaded here, not inside the first turn's time to first token
         engine.phases_ms(reset=True)
     except LiyabError as e:

@@ -25,13 +25,16 @@ class EngineCore:
     def __init__(self, model_dir: Optional[str] = None, *, dtype="bfloat16", device="cuda:0", page_size: int = 16,
                  num_pages: Optional[int] = None, max_tokens: Optional[int] = None, max_requests: int = 64,
                  context_length: Optional[int] = None, use_graphs: bool = True, model=None, config=None,
-                 batch_invariant: bool = False):
+                 batch_invariant: bool = False, weights: Optional[str] = None, rows: Optional[str] = None):
         """`model_dir`: a folder with config.json and model.safetensors (or pass a built
         `model`, see `from_plan`). `num_pages`: pages per cache group; or `max_tokens`: the
         most tokens live requests hold together (rounded up to whole pages per request by the
         caller's accounting). With neither, every request slot can reach the full context.
         `batch_invariant`: a request's bfloat16 logits have the same bits alone and in any batch
-        (kernels chosen from sizes and positions only: slower; float32 is so either way)."""
+        (kernels chosen from sizes and positions only: slower; float32 is so either way).
+        `weights="mxfp4"`: the matrices of attention's and the feed-forwards' products in 4 bits, groups of 32 under a
+        power of two, rounded at load (embeddings, heads, routed experts and what recurrences read stay as they are);
+        `rows="mxfp8"` with it, in bfloat16: these products take their rows in 8 bits."""
         if not torch.cuda.is_available():
             raise KernelError("no GPU is visible: this engine runs on gfx950 only and has no CPU path")
         from ..kernels import ops
@@ -42,8 +45,10 @@ class EngineCore:
         if model is None:
             if model_dir is None:
                 raise InvalidArgument("a model folder or a built model is needed")
-            self.config, self.model = load_model(model_dir, self.dtype, self.device)
+            self.config, self.model = load_model(model_dir, self.dtype, self.device, weights=weights, rows=rows)
         else:
+            if weights is not None or rows is not None:
+                raise InvalidArgument("weights and rows are chosen where a model is built (from_plan, or a model folder)")
             self.config, self.model = config, model
         max_positions = self.model.max_positions
         if context_length is not None:
@@ -74,7 +79,7 @@ class EngineCore:
                  self.storage.bytes_per_token() / 1024.0, self.storage.bytes_allocated() / 2.0 ** 20)
 
     @classmethod
-    def from_plan(cls, plan, tensors, *, dtype="float32", device="cuda:0", **kw) -> "EngineCore":
+    def from_plan(cls, plan, tensors, *, dtype="float32", device="cuda:0", weights: Optional[str] = None, rows: Optional[str] = None, **kw) -> "EngineCore":
         """An engine for a plan and a dict of CPU tensors by name: how a model is built
         without a folder (tests build toy architectures so)."""
         from ..models.decoder import DecoderModel
@@ -82,7 +87,7 @@ class EngineCore:
 
         dt = resolve_dtype(dtype)
         store = WeightStore(dict(tensors), device=device, compute_dtype=dt, name_prefixes=plan.name_prefixes,
-                            ignorable=plan.ignorable)
+                            ignorable=plan.ignorable, products=weights, rows=rows)
         model = DecoderModel(plan, store, dt)
         store.finish()
         return cls(None, dtype=dt, device=device, model=model, config=None, **kw)

@@ -57,6 +57,8 @@ class Mxfp4Matrix:
 
     replayable = True  # (layers that hold it may run from a recorded list: it is its tensor and its sizes)
 
+    eight_bit_rows = False  # a model served with 8-bit rows sets it on its matrices: products by them take `Mxfp8Rows`
+
     def __init__(self, blocks: torch.Tensor, rows: int, width: int):
         if rows < 1 or width < 1:
             raise KernelError(f"a matrix of {rows} x {width}")
@@ -142,9 +144,14 @@ class Mxfp8Rows:
         return self.codes.device
 
     @classmethod
+    def shapes(cls, n: int, width: int):
+        """The shapes of the codes and the scales of n rows."""
+        return (n, _round_up(width, CHUNK)), (n, cls.scale_width(width))
+
+    @classmethod
     def empty(cls, n: int, width: int, device="cuda") -> "Mxfp8Rows":
-        return cls(torch.empty((n, _round_up(width, CHUNK)), dtype=torch.uint8, device=device),
-                   torch.empty((n, cls.scale_width(width)), dtype=torch.uint8, device=device), width)
+        codes, scales = cls.shapes(n, width)
+        return cls(torch.empty(codes, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.uint8, device=device), width)
 
     @classmethod
     def pack(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Mxfp8Rows":

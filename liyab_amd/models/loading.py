@@ -25,13 +25,14 @@ def resolve_dtype(dtype) -> torch.dtype:
     return DTYPES[dtype]
 
 
-def load_model(model_dir: str, dtype="bfloat16", device="cuda:0"):
+def load_model(model_dir: str, dtype="bfloat16", device="cuda:0", weights=None, rows=None):
     """(config, model): the class is chosen by config.json's architecture; all
-    weight problems come as one InvalidModel."""
+    weight problems come as one InvalidModel. `weights` ("mxfp4") and `rows` ("mxfp8"): how matrices that
+    products alone read are kept, and the rows that these products take (`WeightStore`)."""
     config = load_config(model_dir)
     plan = config.plan()
     store = WeightStore.open(model_dir, device=device, compute_dtype=resolve_dtype(dtype),
-                             name_prefixes=plan.name_prefixes, ignorable=plan.ignorable)
+                             name_prefixes=plan.name_prefixes, ignorable=plan.ignorable, products=weights, rows=rows)
     model = DecoderModel(plan, store, resolve_dtype(dtype))
     store.finish()
     return config, model

@@ -12,9 +12,9 @@ from .. import host
 from ..cache.pages import KVSpec
 from ..cache.storage import LayerCache
 from ..errors import Unsupported
-from ..kernels import ops
+from ..kernels import mx, ops
 from .base import PartStepPlan, StepContext, StepFacts, settled
-from .linear import linear, linear_deferred, paged_qkv_takes
+from .linear import linear, linear_deferred, paged_qkv_takes, product_matrix, rows_for
 from .registry import build_part, register_mixer
 
 
@@ -134,9 +134,9 @@ class Attention:
         self.kv_dim = self.n_kv_head * self.head_dim
         qkv_out = self.q_dim + 2 * self.kv_dim
         t = spec.tensors
-        self.qkv_weight = store.fetch(t["qkv_weight"], (qkv_out, self.width), "matrix")
+        self.qkv_weight = product_matrix(store, store.fetch(t["qkv_weight"], (qkv_out, self.width), "matrix"))
         self.qkv_bias = store.fetch(t["qkv_bias"], (qkv_out,), "vector") if "qkv_bias" in t else None
-        self.out_weight = store.fetch(t["out_weight"], (self.width, self.q_dim), "matrix")
+        self.out_weight = product_matrix(store, store.fetch(t["out_weight"], (self.width, self.q_dim), "matrix"))
         self.out_bias = store.fetch(t["out_bias"], (self.width,), "vector") if "out_bias" in t else None
         pos = getattr(spec, "position", None)
         self.position = build_part("position", pos, store, dtype) if pos is not None else None
@@ -161,6 +161,7 @@ class Attention:
         n = h.shape[0]
         ws = ctx.workspace
         group = ctx.groups[cache.group]
+        h = rows_for(self.qkv_weight, h, ctx, "qkv_in_mx")
         if writes_cache and self.position is None and paged_qkv_takes(self.dtype, self.width):
             # the projection's epilogue puts keys and values straight into their pages
             q = ws.get("q", (n, self.q_dim), self.dtype)
@@ -177,8 +178,9 @@ class Attention:
         # with few tokens attention may leave each (token, head) pair's keys cut into splits, for
         # an output projection that is cut over its inner dimension and merges them as it loads
         # (in 32 bits and in the batch-invariant mode: splits by position, for a projection that merges all of them)
+        wide = not isinstance(self.out_weight, mx.Mxfp4Matrix)
         exact = self.dtype == torch.float32 or ops.is_batch_invariant()
-        cut = defer and (self.out_weight.data_ptr() % 16 == 0 if exact else ops.k_parts(n, self.width, self.q_dim) > 1)
+        cut = defer and wide and (self.out_weight.data_ptr() % 16 == 0 if exact else ops.k_parts(n, self.width, self.q_dim) > 1)
         splits = ops.attention(att, q[:, :self.q_dim] if q.shape[1] != self.q_dim else q, cache.k, cache.v, group.block_tables, ctx,
                                n_head=self.n_head, scale=self.scale, window=self.window, splits_ok=cut)
         split = linear_deferred(splits if splits is not None else att, self.out_weight, self.out_bias, ctx, "att_parts", residual) if defer and not exact else None
@@ -187,7 +189,7 @@ class Attention:
         elif split is None:
             if splits is not None:
                 ops.attention_merge(att, splits)
-            linear(att, self.out_weight, self.out_bias, residual=settled(residual))
+            linear(rows_for(self.out_weight, att, ctx, "att_mx"), self.out_weight, self.out_bias, residual=settled(residual))
         return split
 
 

@@ -5,10 +5,10 @@ from __future__ import annotations
 import torch
 
 from ..errors import Unsupported
-from ..kernels import ops
+from ..kernels import mx, ops
 from .base import SplitStream, StepContext, settled
 from .linear import linear
-from .norms import as_tensor
+from .norms import as_tensor, mx_place
 from .registry import register_block, register_connection
 
 
@@ -245,6 +245,8 @@ class SandwichBlock:
         norm = getattr(following, "norm_mixer", None)
         if not isinstance(following, SandwichBlock) or not getattr(norm, "root_mean_square", False) or norm.weight is None or norm.dtype != self.norm_mixer.dtype:
             return False
+        if getattr(following.mixer, "takes_mx_rows", False):
+            return False  # (it reads the norm in 8 bits)
         self.next_weight, self.next_eps = norm.weight, float(norm.eps)
         following.input_normed = True
         return True
@@ -265,18 +267,29 @@ class SandwichBlock:
         if norm_mixer is None or (ffn is not None and norm_ffn is None):
             raise ValueError("a sandwich block has a norm before each sublayer")
 
+    @staticmethod
+    def _normed(norm, part, x, ctx):
+        """What `part` reads of the stream: the norm of its rows, in 8 bits where the part takes them so."""
+        if getattr(part, "takes_mx_rows", False) and hasattr(norm, "mx_rows"):
+            return norm.mx_rows(x, ctx, "block_in_mx")
+        return norm.forward(x, ctx, name="block_in")
+
     def forward(self, x: torch.Tensor, ctx: StepContext, cache, state, writes_cache: bool = True):
         ws, n, d = ctx.workspace, x.shape[0], x.shape[1]
         if ctx.phases is not None:
             ctx.phases.mark(self.mixer_phase)
         # (the block before may have left this block's first norm of the rows where this block's own norm would put it)
-        h = ws.get("block_in", (n, d), self.norm_mixer.dtype) if self.input_normed else self.norm_mixer.forward(x, ctx, name="block_in")
+        if self.input_normed:
+            h = ws.get("block_in", (n, d), self.norm_mixer.dtype)
+        else:
+            h = self._normed(self.norm_mixer, self.mixer, x, ctx)
         y = ws.get("sublayer_out", (n, d), torch.float32)
         self.mixer.forward(h, ctx, cache, state, None, writes_cache=writes_cache, out=y)
         # the update of the rows also takes the next norm of the new rows, where that is a root-mean-square norm too: the feed-forward's
         # own, or, behind the layer's last sublayer, the next layer's first
         chained = (self.next_weight, self.next_eps) if self.next_weight is not None else None
-        fused = self.ffn is not None and getattr(self.norm_ffn, "root_mean_square", False) and self.norm_ffn.weight is not None
+        fused = (self.ffn is not None and getattr(self.norm_ffn, "root_mean_square", False) and self.norm_ffn.weight is not None
+                 and not getattr(self.ffn, "takes_mx_rows", False))
         if fused:
             h = ws.get("block_in", (n, d), self.norm_ffn.dtype)
             ops.gated_norm_add(x, y, self.post_norm_mixer.weight, self.post_norm_mixer.eps, cast_out=h, next_norm=(self.norm_ffn.weight, self.norm_ffn.eps))
@@ -288,7 +301,7 @@ class SandwichBlock:
             if ctx.phases is not None:
                 ctx.phases.mark(self.ffn_phase)
             if not fused:
-                h = self.norm_ffn.forward(x, ctx, name="block_in")
+                h = self._normed(self.norm_ffn, self.ffn, x, ctx)
             k = int(getattr(self.ffn, "rows_a_token", 1))
             y = ws.get("sublayer_rows", (n * k, d), torch.float32) if k > 1 else y
             self.ffn.forward(h, ctx, None, out=y)
@@ -416,7 +429,7 @@ class StreamsBlock:
         self.connect_mixer, self.connect_ffn = connect_mixer, connect_ffn if ffn is not None else None
         self.mixer_phase = getattr(getattr(spec, "mixer", None), "kind", "mixer")
         self.ffn_phase = getattr(getattr(spec, "ffn", None), "kind", "ffn")
-        self.next_norm, self.input_normed = None, False
+        self.next_norm, self.next_mx, self.input_normed = None, False, False
         for part, what in ((mixer, "mixer"), (ffn, "feed-forward")):
             if part is not None and "out" not in part.forward.__code__.co_varnames:
                 raise ValueError(f"a block of several streams needs a {what} that can leave its result to the block (forward(..., out=))")
@@ -436,39 +449,60 @@ class StreamsBlock:
         if not isinstance(following, StreamsBlock) or following.norm_mixer.dtype != self.norm_mixer.dtype:
             return False
         self.next_norm = list(self._reads(following.connect_mixer, following.norm_mixer))
+        self.next_mx = bool(getattr(following.mixer, "takes_mx_rows", False))
         following.input_normed = True
         return True
 
     def enter(self, x: torch.Tensor, embedded: torch.Tensor, ctx: StepContext) -> None:
         """Sets all streams of `x` to the embedding's output and takes the first sublayer's norm of them, for the first block of a model."""
         n, _, d = x.shape
-        ops.streams_update(x, enter=embedded, next_norm=self._reads(self.connect_mixer, self.norm_mixer), out=ctx.workspace.get("block_in", (n, d), self.norm_mixer.dtype))
+        h = ctx.workspace.get("block_in", (n, d), self.norm_mixer.dtype)
+        ops.streams_update(x, enter=embedded, next_norm=self._reads(self.connect_mixer, self.norm_mixer), out=h)
+        if getattr(self.mixer, "takes_mx_rows", False):
+            mx.rows_mx(mx_place(ctx, "block_in_mx", n, d), h)
 
-    def _update(self, x, y, ctx, connection, following, **rows) -> torch.Tensor:
-        """The streams with the sublayer's result; what the following sublayer reads, or None where nobody is known to follow."""
-        n, _, d = x.shape
+    def _update(self, x, y, ctx, connection, following, in_mx, **rows):
+        """The streams with the sublayer's result; what the following sublayer reads (`in_mx`: in 8 bits), or None where nobody is known to follow."""
+        n, S, d = x.shape
+        if following is not None and in_mx and S == 1 and connection is None and following[0] is None and rows.get("n_sum", 1) == 1 and rows.get("identity") is None:
+            # one stream, a plain sum: the addition is the norm's
+            h = mx_place(ctx, "block_in_mx", n, d)
+            stream = x.view(n, d)
+            mx.norm_mx(h, stream, following[1], following[2], add=y, stream=stream)
+            return h
         h = ctx.workspace.get("block_in", (n, d), self.norm_mixer.dtype) if following is not None else None
         mix, give = (connection.mix, connection.give) if connection is not None else (None, None)
         ops.streams_update(x, y=y, mix=mix, add=give, next_norm=following, out=h, **rows)
-        return h
+        if following is None or not in_mx:
+            return h
+        out = mx_place(ctx, "block_in_mx", n, d)
+        mx.rows_mx(out, h)
+        return out
 
     def forward(self, x: torch.Tensor, ctx: StepContext, cache, state, writes_cache: bool = True):
         ws, (n, _, d) = ctx.workspace, x.shape
         if ctx.phases is not None:
             ctx.phases.mark(self.mixer_phase)
-        h = ws.get("block_in", (n, d), self.norm_mixer.dtype)
-        if not self.input_normed:
-            ops.streams_update(x, next_norm=self._reads(self.connect_mixer, self.norm_mixer), out=h)
+        in_mx = bool(getattr(self.mixer, "takes_mx_rows", False))
+        if self.input_normed and in_mx:
+            h = mx_place(ctx, "block_in_mx", n, d)
+        else:
+            h = ws.get("block_in", (n, d), self.norm_mixer.dtype)
+            if not self.input_normed:
+                ops.streams_update(x, next_norm=self._reads(self.connect_mixer, self.norm_mixer), out=h)
         y = ws.get("sublayer_out", (n, d), torch.float32)
         self.mixer.forward(h, ctx, cache, state, None, writes_cache=writes_cache, out=y)
-        h = self._update(x, y, ctx, self.connect_mixer, self._reads(self.connect_ffn, self.norm_ffn) if self.ffn is not None else self.next_norm)
+        if self.ffn is not None:
+            h = self._update(x, y, ctx, self.connect_mixer, self._reads(self.connect_ffn, self.norm_ffn), bool(getattr(self.ffn, "takes_mx_rows", False)))
+        else:
+            self._update(x, y, ctx, self.connect_mixer, self.next_norm, self.next_mx)
         if self.ffn is not None:
             if ctx.phases is not None:
                 ctx.phases.mark(self.ffn_phase)
             k = int(getattr(self.ffn, "rows_a_token", 1))
             y = ws.get("sublayer_rows", (n * k, d), torch.float32) if k > 1 else y
             identity = self.ffn.forward(h, ctx, None, out=y)
-            self._update(x, y, ctx, self.connect_ffn, self.next_norm, n_sum=k, identity=identity)
+            self._update(x, y, ctx, self.connect_ffn, self.next_norm, self.next_mx, n_sum=k, identity=identity)
         return None
 
 

@@ -7,7 +7,8 @@ from typing import Optional
 import torch
 
 from .base import StepContext, settled
-from .linear import linear, linear_deferred
+from .linear import eight_bits, linear, linear_deferred, product_matrix, rows_for
+from .norms import mx_place
 from .registry import register_ffn
 
 
@@ -30,9 +31,9 @@ class DenseFFN:
         if self.activation not in ("gelu_tanh", "gelu_erf"):
             raise ValueError(f"unknown activation '{self.activation}'")
         t = spec.tensors
-        self.up_weight = store.fetch(t["up_weight"], (self.inner, self.width), "matrix")
+        self.up_weight = product_matrix(store, store.fetch(t["up_weight"], (self.inner, self.width), "matrix"))
         self.up_bias = store.fetch(t["up_bias"], (self.inner,), "vector") if "up_bias" in t else None
-        self.down_weight = store.fetch(t["down_weight"], (self.width, self.inner), "matrix")
+        self.down_weight = product_matrix(store, store.fetch(t["down_weight"], (self.width, self.inner), "matrix"))
         self.down_bias = store.fetch(t["down_bias"], (self.width,), "vector") if "down_bias" in t else None
 
     defers = True  # forward(..., defer=True) takes the stream split or whole and may hand it back split
@@ -43,10 +44,10 @@ class DenseFFN:
         stream with the output added comes back as a SplitStream (None: added in place, to
         the stream's own tensor)."""
         inner = ctx.workspace.get("ffn_inner", (h.shape[0], self.inner), self.dtype)
-        linear(h, self.up_weight, self.up_bias, out=inner, activation=self.activation)
+        linear(rows_for(self.up_weight, h, ctx, "ffn_in_mx"), self.up_weight, self.up_bias, out=inner, activation=self.activation)
         split = linear_deferred(inner, self.down_weight, self.down_bias, ctx, "ffn_parts", residual) if defer else None
         if split is None:
-            linear(inner, self.down_weight, self.down_bias, residual=settled(residual))
+            linear(rows_for(self.down_weight, inner, ctx, "ffn_inner_mx"), self.down_weight, self.down_bias, residual=settled(residual))
         return split
 
 
@@ -61,6 +62,11 @@ class ClampedGLU:
     replayable = True
     takes_padding_rows = True
 
+    @property
+    def takes_mx_rows(self) -> bool:
+        """Whether the part's input may be rows in 8 bits."""
+        return eight_bits(self.in_weight)
+
     def __init__(self, spec, store, dtype: torch.dtype):
         self.dtype = dtype
         self.width, self.inner = spec.width, spec.inner
@@ -68,21 +74,25 @@ class ClampedGLU:
         if not self.limit > 0:
             raise ValueError(f"clamped feed-forward: a limit of {self.limit}")
         t = spec.tensors
-        self.in_weight = store.fetch_joined([t["gate"], t["up"]], [(self.inner, self.width)] * 2, "matrix", "rows")
-        self.down_weight = store.fetch(t["down"], (self.width, self.inner), "matrix")
+        self.in_weight = product_matrix(store, store.fetch_joined([t["gate"], t["up"]], [(self.inner, self.width)] * 2, "matrix", "rows"))
+        self.down_weight = product_matrix(store, store.fetch(t["down"], (self.width, self.inner), "matrix"))
 
     def begin(self, h, ctx: StepContext) -> torch.Tensor:
         """The first product, [gate | up] of h in 32 bits: everything of the feed-forward that reads its input. A block whose
         sublayers read one pending norm of the stream runs this before any sublayer adds into the stream."""
         gu = ctx.workspace.get("glu_in", (h.shape[0], 2 * self.inner), torch.float32)
-        linear(h, self.in_weight, None, out=gu)
+        linear(rows_for(self.in_weight, h, ctx, "ffn_in_mx"), self.in_weight, None, out=gu)
         return gu
 
     def finish(self, gu: torch.Tensor, ctx: StepContext, residual: Optional[torch.Tensor], out: Optional[torch.Tensor] = None):
-        from ..kernels import ops
+        from ..kernels import mx, ops
 
-        inner = ctx.workspace.get("ffn_inner", (gu.shape[0], self.inner), self.dtype)
-        ops.glu_clamped(inner, gu, self.limit, self.slope, self.shift)
+        if eight_bits(self.down_weight):
+            inner = mx_place(ctx, "ffn_inner_mx", gu.shape[0], self.inner)
+            mx.glu_mx(inner, gu, "clamped", clamp=(self.limit, self.slope, self.shift))
+        else:
+            inner = ctx.workspace.get("ffn_inner", (gu.shape[0], self.inner), self.dtype)
+            ops.glu_clamped(inner, gu, self.limit, self.slope, self.shift)
         if out is not None:
             linear(inner, self.down_weight, None, out=out)
         else:
@@ -104,6 +114,11 @@ class GatedFFN:
     replayable = True
     takes_padding_rows = True
 
+    @property
+    def takes_mx_rows(self) -> bool:
+        """Whether the part's input may be rows in 8 bits."""
+        return eight_bits(self.in_weight)
+
     def __init__(self, spec, store, dtype: torch.dtype):
         from ..kernels import ops
 
@@ -112,27 +127,30 @@ class GatedFFN:
         if self.activation not in ops.GLU_ACTIVATIONS:
             raise ValueError(f"gated feed-forward: activation '{self.activation}' is not known")
         t = spec.tensors
-        self.in_weight = store.fetch_joined([t["gate"], t["up"]], [(self.inner, self.width)] * 2, "matrix", "rows")
-        self.down_weight = store.fetch(t["down"], (self.width, self.inner), "matrix")
+        self.in_weight = product_matrix(store, store.fetch_joined([t["gate"], t["up"]], [(self.inner, self.width)] * 2, "matrix", "rows"))
+        self.down_weight = product_matrix(store, store.fetch(t["down"], (self.width, self.inner), "matrix"))
 
     def begin(self, h, ctx: StepContext) -> torch.Tensor:
         """The first product, [gate | up] of h in 32 bits: everything of the feed-forward that reads its input. In steps of few rows the
         activation is taken in the product's epilogue: what is handed on are the inner rows then."""
         from ..kernels import ops
 
-        if self.dtype == torch.bfloat16 and ops.glu_in_product_takes(h, self.in_weight):
+        if self.dtype == torch.bfloat16 and isinstance(self.in_weight, torch.Tensor) and ops.glu_in_product_takes(h, self.in_weight):
             inner = ctx.workspace.get("ffn_inner", (h.shape[0], self.inner), self.dtype)
             ops.gemm_glu(inner, h, self.in_weight, self.activation)
             return inner
         gu = ctx.workspace.get("glu_in", (h.shape[0], 2 * self.inner), torch.float32)
-        linear(h, self.in_weight, None, out=gu)
+        linear(rows_for(self.in_weight, h, ctx, "ffn_in_mx"), self.in_weight, None, out=gu)
         return gu
 
     def finish(self, gu: torch.Tensor, ctx: StepContext, residual: Optional[torch.Tensor], out: Optional[torch.Tensor] = None):
-        from ..kernels import ops
+        from ..kernels import mx, ops
 
         inner = gu
-        if gu.shape[1] != self.inner:
+        if eight_bits(self.down_weight):
+            inner = mx_place(ctx, "ffn_inner_mx", gu.shape[0], self.inner)
+            mx.glu_mx(inner, gu, self.activation)
+        elif gu.shape[1] != self.inner:
             inner = ctx.workspace.get("ffn_inner", (gu.shape[0], self.inner), self.dtype)
             ops.glu(inner, gu, self.activation)
         if out is not None:
@@ -157,20 +175,25 @@ class NormedPowersFFN:
     replayable = True
     takes_padding_rows = True
 
+    @property
+    def takes_mx_rows(self) -> bool:
+        """Whether the part's input may be rows in 8 bits."""
+        return eight_bits(self.up_weight)
+
     def __init__(self, spec, store, dtype: torch.dtype):
         self.dtype = dtype
         self.width, self.inner, self.eps = spec.width, spec.inner, float(spec.eps)
         if int(spec.powers) != 3:
             raise ValueError(f"a mix of {spec.powers} powers (3 are taken)")
         t = spec.tensors
-        self.up_weight = store.fetch(t["up"], (self.inner, self.width), "matrix")
+        self.up_weight = product_matrix(store, store.fetch(t["up"], (self.inner, self.width), "matrix"))
         self.act = store.fetch(t["act"], (4,), "vector")
-        self.down_weight = store.fetch(t["down"], (self.width, self.inner), "matrix")
+        self.down_weight = product_matrix(store, store.fetch(t["down"], (self.width, self.inner), "matrix"))
 
     def begin(self, h, ctx: StepContext) -> torch.Tensor:
         """The first product in 32 bits: everything of the feed-forward that reads its input."""
         z = ctx.workspace.get("powers_in", (h.shape[0], self.inner), torch.float32)
-        linear(h, self.up_weight, None, out=z)
+        linear(rows_for(self.up_weight, h, ctx, "ffn_in_mx"), self.up_weight, None, out=z)
         return z
 
     def finish(self, z: torch.Tensor, ctx: StepContext, residual: Optional[torch.Tensor], out: Optional[torch.Tensor] = None):
@@ -179,9 +202,9 @@ class NormedPowersFFN:
         inner = ctx.workspace.get("ffn_inner", (z.shape[0], self.inner), self.dtype)
         ops.normed_powers(inner, z, self.act, self.eps)
         if out is not None:
-            linear(inner, self.down_weight, None, out=out)
+            linear(rows_for(self.down_weight, inner, ctx, "ffn_inner_mx"), self.down_weight, None, out=out)
         else:
-            linear(inner, self.down_weight, None, residual=settled(residual))
+            linear(rows_for(self.down_weight, inner, ctx, "ffn_inner_mx"), self.down_weight, None, residual=settled(residual))
         return None
 
     def forward(self, h, ctx: StepContext, residual: Optional[torch.Tensor], out: Optional[torch.Tensor] = None):

@@ -14,8 +14,9 @@ from typing import Optional
 
 import torch
 
-from ..kernels import ops
-from .norms import Normed
+from ..errors import KernelError
+from ..kernels import mx, ops
+from .norms import Normed, mx_place
 
 
 # Folding the norm into a decode step's products saves a launch of the seven a layer has; every
@@ -55,10 +56,40 @@ def _fuses_exactly(a, w: torch.Tensor, residual) -> bool:
     return ops.is_batch_invariant() and w.dtype == a.norm.dtype == torch.bfloat16 and ops.norm_in_rows_pays(a.n_rows, w.shape[0], a.norm.width)
 
 
+def product_matrix(store, w: torch.Tensor):
+    """What `linear` multiplies by: the matrix as the store keeps matrices for products, in 4 bits (`mx.Mxfp4Matrix`) where the model is served so. For
+    matrices that only `linear` reads."""
+    keep = getattr(store, "for_products", None)
+    return w if keep is None else keep(w)
+
+
+def eight_bits(w) -> bool:
+    """Whether products by this matrix take their rows in 8 bits."""
+    return isinstance(w, mx.Mxfp4Matrix) and w.eight_bit_rows
+
+
+def rows_for(w, h, ctx, name: str):
+    """The rows `h` (a tensor, a pending norm, rows in 8 bits) as products by `w` take them: in 8 bits where they do, in the step's workspace under `name`;
+    `h` itself otherwise."""
+    if not eight_bits(w) or isinstance(h, mx.Mxfp8Rows):
+        return h
+    if isinstance(h, Normed):
+        return h.mx_rows()
+    out = mx_place(ctx, name, h.shape[0], h.shape[1])
+    mx.rows_mx(out, h)
+    return out
+
+
 def linear(a, w: torch.Tensor, bias: Optional[torch.Tensor], *, out: Optional[torch.Tensor] = None,
            residual: Optional[torch.Tensor] = None, activation: str = "none", kv=None) -> None:
     """out = act(a . w^T + bias); with `residual`: residual += a . w^T + bias; with `kv` =
-    (k_cache, v_cache, slots, q_dim): queries to `out`, keys and values into their pages."""
+    (k_cache, v_cache, slots, q_dim): queries to `out`, keys and values into their pages. `w` may be a matrix in 4 bits (`product_matrix`), `a`
+    then rows in 8 bits where it takes them (`rows_for`)."""
+    if isinstance(w, mx.Mxfp4Matrix):
+        if w.eight_bit_rows and not isinstance(a, mx.Mxfp8Rows):
+            raise KernelError("a product by this matrix takes its rows in 8 bits (rows_for)")
+        mx.gemm_mx(a.tensor() if isinstance(a, Normed) else a, w, bias, out=out, residual=residual, activation=activation, kv=kv)
+        return
     if residual is not None:
         epilogue = ops.EPI_RESIDUAL
     elif kv is not None:
@@ -97,6 +128,8 @@ def linear_deferred(a, w: torch.Tensor, bias: Optional[torch.Tensor], ctx, name:
     next product cut this way writes its own under another name."""
     from .base import SplitStream
 
+    if isinstance(w, mx.Mxfp4Matrix):
+        return None
     if ops.is_batch_invariant():
         return None  # no cut over K: its parts would follow the step's size
     a = a.tensor() if isinstance(a, Normed) else a

@@ -6,9 +6,15 @@ from typing import Optional
 
 import torch
 
-from ..kernels import ops
+from ..kernels import mx, ops
 from .base import StepContext
 from .registry import register_norm
+
+
+def mx_place(ctx: StepContext, name: str, n: int, width: int) -> mx.Mxfp8Rows:
+    """Places for n rows of `width` values in 8 bits, in the step's workspace under `name`."""
+    codes, scales = mx.Mxfp8Rows.shapes(n, width)
+    return mx.Mxfp8Rows(ctx.workspace.get(name, codes, torch.uint8), ctx.workspace.get(name + "_scales", scales, torch.uint8), width)
 
 
 class Normed:
@@ -20,7 +26,7 @@ class Normed:
         self.norm, self.x, self.ctx, self.rows, self.name = norm, x, ctx, rows, name
         # x: the rows [n, d], or a sum of planes [parts, n, d] for a norm that `takes_planes`
         self.n_rows = x.shape[-2] if rows is None else (n_rows if n_rows is not None else rows.numel())
-        self._tensor = None
+        self._tensor = self._mx_rows = None
 
     @property
     def shape(self):
@@ -34,6 +40,17 @@ class Normed:
         if self._tensor is None:
             self._tensor = self.norm.forward(self.x, self.ctx, rows=self.rows, n_rows=self.n_rows, name=self.name)
         return self._tensor
+
+    def mx_rows(self) -> mx.Mxfp8Rows:
+        """The rows in 8 bits: from the norm itself where it leaves them so, else rounded from its rows."""
+        if self._mx_rows is None:
+            whole = self.rows is None and self.x.dim() == 2 and self._tensor is None
+            if whole and hasattr(self.norm, "mx_rows"):
+                self._mx_rows = self.norm.mx_rows(self.x, self.ctx, self.name + "_mx")
+            else:
+                self._mx_rows = mx_place(self.ctx, self.name + "_mx", *self.shape)
+                mx.rows_mx(self._mx_rows, self.tensor())
+        return self._mx_rows
 
 
 def as_tensor(h) -> torch.Tensor:
@@ -81,6 +98,12 @@ class LayerNorm:
         ops.layernorm(out, x, self.weight, self.bias, self.eps, rows=rows)
         return out
 
+    def mx_rows(self, x: torch.Tensor, ctx: StepContext, name: str) -> mx.Mxfp8Rows:
+        """The norm of every row of x [n, width] in 8 bits."""
+        out = mx_place(ctx, name, x.shape[0], self.width)
+        mx.norm_mx(out, x, self.weight, self.eps, bias=self.bias, centred=True)
+        return out
+
 
 register_norm("layernorm", LayerNorm)
 
@@ -116,6 +139,12 @@ class RMSNorm:
             ops.streams_update(x, next_norm=(None, self.weight, self.eps), out=out, rows=rows)
         else:
             ops.rmsnorm(out, x, self.weight, self.eps, rows=rows)
+        return out
+
+    def mx_rows(self, x: torch.Tensor, ctx: StepContext, name: str, add: Optional[torch.Tensor] = None) -> mx.Mxfp8Rows:
+        """The norm of every row of x [n, width] in 8 bits; with `add`, x += add first."""
+        out = mx_place(ctx, name, x.shape[0], self.width)
+        mx.norm_mx(out, x, self.weight, self.eps, add=add, stream=x if add is not None else None)
         return out
 
 

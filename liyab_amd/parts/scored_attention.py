@@ -14,7 +14,7 @@ from ..errors import Unsupported
 from ..kernels import ops
 from .attention import AttentionStepPlanner
 from .base import StepContext, settled
-from .linear import linear
+from .linear import eight_bits, linear, product_matrix, rows_for
 from .norms import as_tensor
 from .registry import register_mixer
 
@@ -121,7 +121,7 @@ class ScoredAttention:
             srcs.append(t["gate"])
             shapes.append((H * V, d))
             at += H * V
-        self.in_weight = store.fetch_joined(srcs, shapes, "matrix", "rows")
+        self.in_weight = product_matrix(store, store.fetch_joined(srcs, shapes, "matrix", "rows"))
         # biases on the projections of queries, keys and values: one vector over the joint product's columns, zeros for the gate's
         self.in_bias = None
         if getattr(spec, "biased", False):
@@ -152,6 +152,7 @@ class ScoredAttention:
             P = self.row_dim = -(-max(D, V) // 8) * 8
             w = self.out_weight
             self.out_weight = store.derived(("padded_heads", t["out"].name, P), lambda: torch.nn.functional.pad(w.view(d, H, V), (0, P - V)).reshape(d, H * P).contiguous())
+        self.out_weight = product_matrix(store, self.out_weight)
         per_q, per_k = (H * D, G * D) if self.norm_rows else (D, D)
         normed = spec.qk_norm or self.norm_rows
         if spec.qk_norm and not getattr(spec, "qk_norm_weights", True):
@@ -181,6 +182,11 @@ class ScoredAttention:
             self.bias_table = store.derived(("distance_bias", t["rel"].name, far),
                                             lambda: rel[torch.from_numpy(distance_rows(rows, far)).to(rel.device)].contiguous())
 
+    @property
+    def takes_mx_rows(self) -> bool:
+        """Whether the part's input may be rows in 8 bits."""
+        return eight_bits(self.in_weight)
+
     def _shared_values(self, ws, n: int) -> dict:
         if not self.value_mix:
             return {}
@@ -208,7 +214,7 @@ class ScoredAttention:
         group = ctx.groups[cache.group]
         if proj is None:
             proj = ws.get("scored_in", (n, self.in_weight.shape[0]), torch.float32)
-            linear(h, self.in_weight, self.in_bias, out=proj)
+            linear(rows_for(self.in_weight, h, ctx, "scored_in_mx"), self.in_weight, self.in_bias, out=proj)
         P = self.row_dim
         q = ws.get("scored_q", (n, H * (P or D)), self.dtype)
         if writes_cache == self.kv_shared:
@@ -240,11 +246,11 @@ class ScoredAttention:
             ops.attention_scored(att, q, cache.k, cache.v, group.block_tables, ctx, n_head=H, scale=self.scale, softcap=self.softcap,
                                  window=self.window, bias_table=self.bias_table, gate=gate, sinks=self.sinks, keep_first=self.keep_first)
         if out is not None and add:
-            linear(att, self.out_weight, None, residual=out)
+            linear(rows_for(self.out_weight, att, ctx, "att_mx"), self.out_weight, None, residual=out)
         elif out is not None:
-            linear(att, self.out_weight, None, out=out)
+            linear(rows_for(self.out_weight, att, ctx, "att_mx"), self.out_weight, None, out=out)
         else:
-            linear(att, self.out_weight, None, residual=settled(residual))
+            linear(rows_for(self.out_weight, att, ctx, "att_mx"), self.out_weight, None, residual=settled(residual))
         return None
 
 

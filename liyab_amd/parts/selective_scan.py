@@ -12,7 +12,7 @@ from ..errors import Unsupported
 from ..kernels import ops
 from .base import StepContext, settled
 from .delta_rule import own_state
-from .linear import linear
+from .linear import eight_bits, linear, product_matrix, rows_for
 from .norms import as_tensor
 from .registry import register_mixer
 
@@ -36,7 +36,7 @@ class SelectiveScan:
         if self.taps < 1:
             raise ValueError(f"selective scan: a convolution of {self.taps} taps")
         t = spec.tensors
-        self.in_weight = store.fetch(t["in"], (2 * W, d), "matrix")
+        self.in_weight = product_matrix(store, store.fetch(t["in"], (2 * W, d), "matrix"))
         self.conv = store.fetch(t["conv"], (W, self.taps), "vector")
         self.conv_bias = store.fetch(t["conv_bias"], (W,), "vector")
         self.x_weight = store.fetch(t["x"], (R + 2 * N, W), "matrix")
@@ -50,7 +50,12 @@ class SelectiveScan:
         # [states, channels], times log2(e): a decay is 2^(dt a)
         self.a2 = store.derived(("decay_rates", t["A_log"].name), lambda: (a_log.double().exp() * -math.log2(math.e)).t().float().contiguous())
         self.skip = store.fetch(t["D"], (W,), "vector")
-        self.out_weight = store.fetch(t["out"], (d, W), "matrix")
+        self.out_weight = product_matrix(store, store.fetch(t["out"], (d, W), "matrix"))
+
+    @property
+    def takes_mx_rows(self) -> bool:
+        """Whether the part's input may be rows in 8 bits."""
+        return eight_bits(self.in_weight)
 
     def _floats(self) -> int:
         return (self.n_state + self.taps - 1) * self.inner
@@ -65,11 +70,11 @@ class SelectiveScan:
                 out: Optional[torch.Tensor] = None):
         if not writes_cache:
             raise Unsupported("selective scan: a run that leaves the state as it found it is not supported")
-        h = as_tensor(h)
+        h = h if self.takes_mx_rows else as_tensor(h)
         n, ws, W, N = h.shape[0], ctx.workspace, self.inner, self.n_state
         own = own_state(state, self._floats())
         proj = ws.get("selective_in", (n, 2 * W), torch.float32)
-        linear(h, self.in_weight, None, out=proj)
+        linear(rows_for(self.in_weight, h, ctx, "selective_in_mx"), self.in_weight, None, out=proj)
         raw, z = proj[:, :W], proj[:, W:]
         x = ws.get("selective_x", (n, W), self.dtype)
         ops.conv_act(x, raw, self.conv, self.conv_bias, own.state, own.offset + N * W, ctx)
@@ -79,9 +84,9 @@ class SelectiveScan:
         # (the walk also keeps the step's last rows of x in the slot's ring: the convolution, which reads the ring, has run)
         ops.selective_scan(y, x, low, z, self.dt_weight, self.dt_weight_t, self.dt_bias, self.a2, self.skip, own, raw, self.taps, ctx)
         if out is not None:
-            linear(y, self.out_weight, None, out=out)
+            linear(rows_for(self.out_weight, y, ctx, "selective_out_mx"), self.out_weight, None, out=out)
         else:
-            linear(y, self.out_weight, None, residual=settled(residual))
+            linear(rows_for(self.out_weight, y, ctx, "selective_out_mx"), self.out_weight, None, residual=settled(residual))
         return None
 
 

@@ -10,7 +10,9 @@ that lists missing tensors, wrong shapes and names nobody asked for.
 Precision: matrices and tables go to the device in the compute dtype of the
 path (bfloat16 for serving, float32 for the 32-bit path); vectors (norm
 weights, biases) are float32 on both paths; integer tensors become int32.
-A tensor is converted once, at load, and stays resident.
+A tensor is converted once, at load, and stays resident. With `products="mxfp4"` the matrices that parts
+hand to products alone (`for_products`) are kept in 4 bits instead, rounded from the compute dtype's, and with
+`rows="mxfp8"` these products take their rows in 8 bits.
 """
 
 from __future__ import annotations
@@ -22,7 +24,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 import torch
 
 from ..config.plan import TensorSource
-from ..errors import InvalidModel
+from ..errors import InvalidArgument, InvalidModel, Unsupported
 from .safetensors_io import SafetensorsFile
 
 WEIGHTS_FILE = "model.safetensors"
@@ -38,7 +40,19 @@ class WeightStore:
         name_prefixes: Sequence[str] = ("",),
         ignorable: Sequence[str] = (),
         origin: str = "<memory>",
+        products: Optional[str] = None,
+        rows: Optional[str] = None,
     ):
+        if products not in (None, "mxfp4"):
+            raise InvalidArgument(f"weights '{products}' are not one of mxfp4 (4 bits in groups of 32), or None for the compute dtype")
+        if rows not in (None, "mxfp8"):
+            raise InvalidArgument(f"rows '{rows}' are not one of mxfp8 (8 bits in groups of 32), or None for the compute dtype")
+        if rows is not None and products is None:
+            raise InvalidArgument("rows in 8 bits are for products by matrices in 4 bits (weights 'mxfp4')")
+        if rows is not None and compute_dtype == torch.float32:
+            raise InvalidArgument("rows in 8 bits are for the bfloat16 path: the float32 path keeps its rows in 32 bits")
+        self.products, self.rows = products, rows
+        self._in_4_bits: Dict[tuple, tuple] = {}
         self._tensors = tensors
         self.device = torch.device(device)
         self.compute_dtype = compute_dtype
@@ -90,6 +104,20 @@ class WeightStore:
         if hit is None:
             hit = self._derived[key] = make()
         return hit
+
+    def for_products(self, w: torch.Tensor):
+        """The matrix w [out, in] as products read it: itself, or in 4 bits. The same matrix gives the same object (layers that share their weights share it)."""
+        if self.products is None:
+            return w
+        from ..kernels.mx import Mxfp4Matrix
+
+        key = (w.data_ptr(), tuple(w.shape))
+        hit = self._in_4_bits.get(key)
+        if hit is None:
+            m = Mxfp4Matrix.quantize(w)
+            m.eight_bit_rows = self.rows is not None
+            hit = self._in_4_bits[key] = (w, m)  # (with w: its address stays its own)
+        return hit[1]
 
     def fetch(self, src: TensorSource, shape: Sequence[int], role: str, keep: bool = True) -> Optional[torch.Tensor]:
         """The tensor `src` names, on the device, in working layout and dtype.
@@ -169,6 +197,8 @@ class WeightStore:
         """Raises one InvalidModel naming every missing, mis-shaped and
         unexpected tensor, or returns when there is none."""
         unexpected = self.unexpected()
+        if self.products is not None and not self._in_4_bits and not self._missing and not self._wrong:
+            raise Unsupported(f"weights '{self.products}': none of this model's parts has a matrix that products alone read")
         if not (self._missing or self._wrong or unexpected):
             return
         lines = [f"the weights in '{self.origin}' do not fit the configuration:"]
