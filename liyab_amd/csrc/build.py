@@ -47,6 +47,7 @@ FILE_FLAGS = {
     "attention_prefill_direct.hip": VGPR_MFMA,
     "attention_rows.hip": VGPR_MFMA,
     "gemm_simple.hip": VGPR_MFMA,
+    "mx_tiles.hip": VGPR_MFMA,
 }
 
 

@@ -239,30 +239,32 @@ static int launch_product(const MxRowsIn& in, const uint8_t* blocks, int M, int 
 // The workgroups' shapes: tiles of 16 rows x strips of 16 columns, and the tiles of mx_tiles.hip.
 enum : int { kShape1x1 = 11, kShape1x2 = 12, kShape2x1 = 21, kShape2x2 = 22, kShape2x4 = 24, kShape4x1 = 41, kShape4x2 = 42, kShape4x4 = 44 };
 
-// The shape whose rounds of workgroups take the least time: `us` is what one round takes at 4,096 k (bfloat16 / 8-bit rows; measured over matrices that are
-// not in the caches, 24 to 512 rows of 1,024 to 16,384 columns), `round` how many workgroups run side by side. A round's time grows with K
-// much the same in all of them. Up to 16 rows, where the matrix's bytes set the pace: 16 waves a strip while every strip has a compute unit of its own
-// (us, 16 waves / 8 waves on two strips: 1 row 1,600 x 6,400 5.0 / 6.7, 8 rows 4,096 x 4,096 5.3 / 6.3, 1 row 4,096 x 16,384 9.7 / 13.6), two
-// strips beyond (1 row 16,384 x 4,096 12.4 / 10.1, 8 rows 6,400 x 1,600 6.2 / 4.5). `fixed`: eight waves whatever the rows, so that a row's sums
-// have one order.
-static int choose_shape(int kind, bool fixed, int M, int N) {
+// The shape that takes the least time: `fixed` and another `round` for each round of 256 workgroups, in us at 4,096 k (bfloat16 / 8-bit rows; measured over
+// matrices that are not in the caches, 24 to 2,048 rows of 768 to 16,384 columns; K changes them all much alike). The shapes of this file fill a compute unit
+// each; the smaller tiles leave room for others, so their rounds run into each other. What it chooses between, us: 512 rows 4,096 x 4,096 4x4 / 64 x 128
+// / 128 x 128 bfloat16 32 / 27 / 38, 8 bits 30 / 16 / 22; 2,048 rows 4,096 x 4,096 64 x 128 / 128 x 128 / 256 x 256 bfloat16 68 / 65 / 85, 8 bits 40 / 36 / 53, 16,384 x
+// 4,096 258 / 226 / 186, 147 / 135 / 112; 64 rows 4,096 x 4,096 2x1 / 4x1 / 2x4 12.8 / 10.6 / 10.8, 128 rows 2x1 / 2x4 / 4x4 22.8 / 10.6 / 16.4. Up to 16 rows the matrix's
+// bytes set the pace: 16 waves a strip while every strip has a compute unit of its own (us, 16 waves / 8 waves on two strips: 1 row 1,600 x 6,400 5.0 / 6.7, 8
+// rows 4,096 x 4,096 5.3 / 6.3, 1 row 4,096 x 16,384 9.7 / 13.6), two strips beyond (1 row 16,384 x 4,096 12.4 / 10.1, 8 rows 6,400 x 1,600 6.2 / 4.5).
+// `same_bits`: eight waves whatever the rows, so that a row's sums have one order.
+static int choose_shape(int kind, bool same_bits, int M, int N) {
     const int strips = mx_strips(N);
-    if (M <= 16) return !fixed && strips <= 256 ? kShape1x1 : kShape1x2;
+    if (M <= 16) return !same_bits && strips <= 256 ? kShape1x1 : kShape1x2;
     struct Shape {
-        int id, rows, columns, round;
-        float us[2];
+        int id, rows, columns;
+        float fixed[2], round[2];
     };
     static const Shape shapes[] = {
-        {kShape2x1, 32, 16, 256, {7.6f, 7.0f}},   {kShape2x2, 32, 32, 256, {9.0f, 8.5f}},    {kShape4x1, 64, 16, 256, {9.7f, 9.7f}},
-        {kShape2x4, 32, 64, 256, {10.6f, 11.0f}}, {kShape4x2, 64, 32, 256, {12.1f, 12.4f}},  {kShape4x4, 64, 64, 256, {16.4f, 16.8f}},
-        {kMxTile128, 128, 128, 512, {57.0f, 46.0f}}, {kMxTile256, 256, 256, 256, {97.0f, 86.0f}},
+        {kShape2x1, 32, 16, {0, 0}, {7.6f, 7.0f}},       {kShape2x2, 32, 32, {0, 0}, {9.0f, 8.5f}},        {kShape4x1, 64, 16, {0, 0}, {9.7f, 9.7f}},
+        {kShape2x4, 32, 64, {0, 0}, {10.6f, 11.0f}},     {kShape4x2, 64, 32, {0, 0}, {12.1f, 12.4f}},      {kShape4x4, 64, 64, {0, 0}, {16.4f, 16.8f}},
+        {kMxTile64, 64, 128, {13.5f, 8.5f}, {13.6f, 8.0f}}, {kMxTile128, 128, 128, {10.5f, 10.0f}, {27.0f, 15.0f}}, {kMxTile256, 256, 256, {0, 0}, {92.0f, 56.0f}},
     };
     int best = kShape4x4;
     float least = 3e38f;
     for (const Shape& s : shapes) {
-        if (s.id < 10 && (fixed || M <= 64)) continue;
+        if (s.id < 10 && (same_bits || M <= 64)) continue;
         const int64_t groups = (static_cast<int64_t>(M) + s.rows - 1) / s.rows * ((N + s.columns - 1) / s.columns);
-        const float us = static_cast<float>((groups + s.round - 1) / s.round) * s.us[kind == kRowsMx];
+        const float us = s.fixed[kind == kRowsMx] + static_cast<float>((groups + 255) / 256) * s.round[kind == kRowsMx];
         if (us < least) least = us, best = s.id;
     }
     return best;
@@ -283,6 +285,7 @@ static int product_of_shape(int shape, const MxRowsIn& in, const uint8_t* blocks
             case kShape4x1: return launch_product<ROWS, 4, 1, 1, 8>(in, blocks, M, N, K, epi, stream);
             case kShape4x2: return launch_product<ROWS, 4, 2, 1, 8>(in, blocks, M, N, K, epi, stream);
             case kShape4x4: return launch_product<ROWS, 4, 4, 1, 8>(in, blocks, M, N, K, epi, stream);
+            case kMxTile64:
             case kMxTile128:
             case kMxTile256: return launch_mx_tiles(ROWS, shape, in, blocks, M, N, K, epi, stream);
             default: return fail(1, "mx_product: unknown shape %d", shape);
