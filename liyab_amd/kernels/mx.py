@@ -98,10 +98,11 @@ class Mxfp4Matrix:
 
     @classmethod
     def pack(cls, codes: torch.Tensor, scales: torch.Tensor, width: int) -> "Mxfp4Matrix":
-        """From plain rows: codes uint8 [out, ceil(width / 2)], two numbers a byte, the first in the low half, and scales [out, ceil(width / 32)]."""
+        """From plain rows: codes uint8 [out, ceil(width / 2)], two numbers a byte, the first in the low half (or whole groups, [out, 16 ceil(width / 32)],
+        where what lies behind the width does not count), and scales [out, ceil(width / 32)]."""
         codes, scales = _bytes(codes, "codes"), _bytes(scales, "scales")
-        if width < 1 or codes.shape[1] != -(-width // 2) or tuple(scales.shape) != (codes.shape[0], -(-width // GROUP)) or scales.device != codes.device:
-            raise KernelError(f"a 4-bit matrix of width {width} needs codes [out, {-(-width // 2)}] and scales [out, {-(-width // GROUP)}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
+        if width < 1 or codes.shape[1] not in (-(-width // 2), -(-width // GROUP) * (GROUP // 2)) or tuple(scales.shape) != (codes.shape[0], -(-width // GROUP)) or scales.device != codes.device:
+            raise KernelError(f"a 4-bit matrix of width {width} needs codes [out, {-(-width // 2)}] or [out, {-(-width // GROUP) * (GROUP // 2)}] and scales [out, {-(-width // GROUP)}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
         out = cls._empty(codes.shape[0], width, codes.device)
         with torch.cuda.device(codes.device):
             _lib.call("liyab_mx_pack", out.blocks.data_ptr(), codes.data_ptr(), _rows(codes, "codes"), scales.data_ptr(), _rows(scales, "scales"), out.rows, width, _stream())

@@ -268,6 +268,22 @@ def test_quantized_matrices_are_the_formats(mx, n, d, dtype):
     assert torch.equal(got.dense(torch.bfloat16).float().nan_to_num(5.0)[torch.from_numpy(fine)], dense.nan_to_num(5.0)[torch.from_numpy(fine)])
 
 
+@pytest.mark.parametrize("n,d", [(3, 31), (5, 130), (196, 279), (16, 257), (4, 64)])
+def test_packed_rows_of_whole_groups(mx, n, d):
+    """Rows of codes may come as whole groups of 32; what lies behind the width does not count."""
+    g = torch.Generator().manual_seed(n * d)
+    groups = -(-d // 32)
+    codes = torch.randint(0, 256, (n, 16 * groups), generator=g, dtype=torch.uint8)
+    scales = torch.randint(100, 140, (n, groups), generator=g, dtype=torch.uint8)
+    plain = codes[:, : -(-d // 2)].clone()
+    if d % 2:
+        plain[:, -1] &= 15
+    whole = mx.Mxfp4Matrix.pack(codes.to(DEV), scales.to(DEV), d)
+    assert torch.equal(whole.blocks, mx.Mxfp4Matrix.pack(plain.to(DEV), scales.to(DEV), d).blocks)
+    with pytest.raises(KernelError):
+        mx.Mxfp4Matrix.pack(torch.zeros(n, 16 * groups + 1, dtype=torch.uint8, device=DEV), scales.to(DEV), d)
+
+
 def check_rows(out, codes, scales, what):
     """Codes and bytes of rows, and zeros behind their width."""
     n, d = codes.shape
