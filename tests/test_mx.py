@@ -1,12 +1,16 @@
 """Microscaling formats without a GPU: the plain implementation's own numbers, and what the operators refuse."""
 
 import math
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
 import torch
 
 import plain_mx
+from liyab_amd.csrc import build
 from liyab_amd.errors import KernelError
 from liyab_amd.kernels import mx
 
@@ -54,3 +58,32 @@ def test_matrices_of_no_size_are_refused(rows, width):
 def test_places_of_rows(width, codes, scales):
     """Rows of codes are whole chunks of 128, rows of scales whole pieces of 16 bytes that hold a byte for each group of the chunks."""
     assert mx._round_up(width, mx.CHUNK) == codes and mx.Mxfp8Rows.scale_width(width) == scales and scales >= codes // 32
+
+
+@pytest.mark.parametrize("source", ["mx_product.hip", "mx_tiles.hip"])
+def test_the_products_waits_are_counted(source, tmp_path):
+    """Both products keep loads in flight across their waits. A spilled register would be a load that the counts do not know of; and the tiles' loop waits for
+    no load but the stage that it needs next, whatever the compiler makes of its reads from LDS."""
+    hipcc = build.hipcc_path()
+    if hipcc is None:
+        pytest.skip("hipcc was not found")
+    out = tmp_path / "kernels.s"
+    r = subprocess.run([hipcc, *build.FLAGS, *build.FILE_FLAGS.get(source, []), "-I", build.CSRC, "--cuda-device-only", "-Rpass-analysis=kernel-resource-usage", "-S",
+                        os.path.join(build.CSRC, source), "-o", str(out)], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-2000:]
+    kernels = re.split(r"Function Name: ", r.stderr)[1:]
+    assert kernels
+    for k in kernels:
+        spilled, scratch = (int(re.search(what + r": (\d+)", k)[1]) for what in ("VGPRs Spill", r"ScratchSize \[bytes/lane\]"))
+        assert spilled == 0 and scratch == 0, f"{k.split()[0]}: {spilled} registers spilled, {scratch} bytes of scratch a lane"
+    if source == "mx_tiles.hip":
+        tiles = re.findall(r"(?ms)^_ZN5liyab14mx_tile_kernel\S*:.*?^\.Lfunc_end", out.read_text())
+        assert len(tiles) == 54
+        for t in tiles:
+            # from the first product to the last; a stage's loads are the rows', the blocks' and one of scales
+            loop = t[t.index("v_mfma"):t.rindex("v_mfma")]
+            counts = {int(n) for n in re.findall(r"vmcnt\((\d+)\)", loop)}
+            stage = re.match(r"_ZN5liyab14mx_tile_kernelILi(\d)ELi(\d)ELi(\d)ELi(\d)ELi(\d)E", t)
+            mx_rows, wm, wn, tm, tn = int(stage[1]) == 2, *(int(stage[i]) for i in range(2, 6))
+            loads = wm * tm * 16 // 8 // (wm * wn) + wn * tn * (1024 if mx_rows else 512) // 1024 // (wm * wn) + 1
+            assert counts == {loads}, f"{t.split(':')[0]}: waits until {sorted(counts)} loads are left, a stage has {loads}"
