@@ -309,7 +309,9 @@ extern "C" int liyab_mx_product(const void* a, int64_t lda, const void* a_scales
     LIYAB_REQUIRE(reinterpret_cast<uintptr_t>(a) % 16 == 0 && reinterpret_cast<uintptr_t>(blocks) % 16 == 0, "mx_product: operands start on 16-byte boundaries");
     const MxRowsIn in{a, lda, static_cast<const uint8_t*>(a_scales), lds};
     const uint8_t* const b = static_cast<const uint8_t*>(blocks);
+    if (shape == 0 && (lda >= (int64_t{1} << 22) || K >= (1 << 22))) shape = -1;  // (a tile's rows are found by 32-bit offsets)
     if (rows == kRowsMx) {
+        LIYAB_REQUIRE(reinterpret_cast<uintptr_t>(a_scales) % 4 == 0, "mx_product: scales start on 4-byte boundaries");  // (a load into LDS takes four)
         LIYAB_REQUIRE(a_scales && lda >= static_cast<int64_t>(mx_chunks(K)) * kMxChunk && lda % 16 == 0 && lds >= mx_chunks(K) * 4, "mx_product: rows in 8 bits are padded to %d codes",
                       mx_chunks(K) * kMxChunk);
         return product_of_shape<kRowsMx>(shape > 0 ? shape : choose_shape(rows, shape < 0, M, N), in, b, M, N, K, *epi, stream);

@@ -128,8 +128,8 @@ class Mxfp8Rows:
             raise KernelError(f"rows of {width} values in 8 bits need contiguous uint8 codes [n, {_round_up(max(width, 1), CHUNK)}] and scales "
                               f"[n, {self.scale_width(max(width, 1))}], got {tuple(codes.shape)} {codes.dtype} and {tuple(scales.shape)} {scales.dtype}")
         _dev(codes, "codes")
-        if codes.data_ptr() % 16:
-            raise KernelError("codes must start on a 16-byte boundary")
+        if codes.data_ptr() % 16 or scales.data_ptr() % 16:
+            raise KernelError("codes and scales must start on 16-byte boundaries")
         self.index = codes.get_device()
 
     @staticmethod

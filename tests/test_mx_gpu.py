@@ -185,6 +185,31 @@ def test_rows_anywhere_in_memory(mx, M, K, shift, kind):
     within(out, av @ wv.T, sums_bound(av, wv, np.zeros(50), K), kind)
 
 
+def test_rows_far_apart(mx):
+    """Rows whose places pass 32 bits: tiles, which find theirs by 32-bit offsets, are not chosen, and not taken."""
+    from liyab_amd.errors import KernelError
+
+    M, N, K, stride = 300, 256, 128, (1 << 22) + 8
+    w, wv = matrix(mx, N, K)
+    a = torch.empty(M * stride, dtype=torch.bfloat16, device=DEV).view(M, stride)[:, 64:64 + K]
+    a.copy_(rnd(M, K, dtype=torch.bfloat16))
+    av = a.double().cpu().numpy()
+    out = torch.empty(M, N, device=DEV)
+    mx.gemm_mx(a, w, None, out=out)
+    within(out, av @ wv.T, sums_bound(av, wv, np.zeros(N), K), "far apart")
+    with pytest.raises(KernelError):
+        mx.gemm_mx(a, w, None, out=out, shape=1)
+
+
+def test_scales_between_pieces_are_refused(mx):
+    from liyab_amd.errors import KernelError
+
+    codes, scales = mx.Mxfp8Rows.shapes(70, 256)
+    flat = torch.zeros(70 * scales[1] + 16, dtype=torch.uint8, device=DEV)
+    with pytest.raises(KernelError):
+        mx.Mxfp8Rows(torch.zeros(codes, dtype=torch.uint8, device=DEV), flat[1:1 + 70 * scales[1]].view(scales), 256)
+
+
 @pytest.mark.parametrize("kind", ["bfloat16", "float32", "mxfp8"])
 @pytest.mark.parametrize("M,H,Hkv,hd,K,page", [(1, 3, 3, 16, 64, 4), (33, 6, 3, 64, 128, 16), (20, 5, 1, 80, 1600, 16), (150, 4, 2, 32, 200, 48)])
 def test_products_write_pages(mx, M, H, Hkv, hd, K, page, kind):
