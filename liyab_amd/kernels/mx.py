@@ -173,6 +173,15 @@ def _check_out(out: Mxfp8Rows, n: int, d: int, what: str) -> None:
         raise KernelError(f"{what}: the rows have places for [{out.n}, {out.width}], not [{n}, {d}]")
 
 
+def _stride(t: torch.Tensor, what: str) -> int:
+    """`ops._rows`, asking the usual rows less (0.4 us a tensor of a call's 8)."""
+    if t.is_cuda and t.dim() == 2:
+        ld, step = t.stride()
+        if step == 1 and ld >= t.shape[1]:
+            return ld
+    return _rows(t, what)
+
+
 def _stream_on(index: int) -> int:
     """The stream that launches go to (`ops._stream`; asked for without the objects that torch makes around it, 2 us of a call)."""
     return ops._pinned_stream if ops._pinned_stream is not None else torch._C._cuda_getCurrentRawStream(index)
@@ -197,7 +206,7 @@ def _on(what: str, index: int, *tensors) -> int:
 
 def rows_mx(out: Mxfp8Rows, x: torch.Tensor) -> None:
     """out = x [n, d] (float32 or bfloat16, rows contiguous) in 8 bits."""
-    ldx = _rows(x, "x")
+    ldx = _stride(x, "x")
     _check_out(out, x.shape[0], x.shape[1], "rows_mx")
     stream = _on("rows_mx", out.index, x)
     if out.n == 0:
@@ -209,7 +218,7 @@ def rows_mx(out: Mxfp8Rows, x: torch.Tensor) -> None:
 def glu_mx(out: Mxfp8Rows, gu: torch.Tensor, activation: str, clamp=None) -> None:
     """out = act(G) * U in 8 bits; gu float32 [n, 2 * d] = [G | U]; act "silu" or "gelu_tanh", or "clamped" with clamp = (limit, slope, shift): g *
     sigmoid(slope * g) * (u + shift), g = min(G, limit), u = clamp(U, -limit, limit) (`ops.glu`, `ops.glu_clamped`)."""
-    ld = _rows(gu, "gu")
+    ld = _stride(gu, "gu")
     n, d2 = gu.shape
     if gu.dtype != torch.float32 or d2 != 2 * out.width:
         raise KernelError(f"glu_mx: needs float32 [n, {2 * out.width}], got {tuple(gu.shape)} {gu.dtype}")
@@ -268,7 +277,7 @@ def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[to
             raise KernelError(f"gemm_mx: rows of {a.width} values, a matrix of width {K}")
         lda, scales, lds = operand.shape[1], a.scales.data_ptr(), a.scales.shape[1]
     else:
-        lda, operand, scales, lds, dtype = _rows(a, "a"), a, None, 0, a.dtype
+        lda, operand, scales, lds, dtype = _stride(a, "a"), a, None, 0, a.dtype
         M, width = a.shape
         if width != K or (dtype is not torch.bfloat16 and dtype is not torch.float32):
             raise KernelError(f"gemm_mx: a {tuple(a.shape)} {dtype} does not fit a matrix of {N} x {K}")
@@ -281,11 +290,11 @@ def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[to
         if residual is not None:
             if residual.dtype is not torch.float32 or residual.shape != (M, N):
                 raise KernelError("gemm_mx: needs a float32 residual [M, N]")
-            e = _lib.EpiParams(EPI_RESIDUAL, F32, _ptr(bias), None, 0, residual.data_ptr(), _rows(residual, "residual"))
+            e = _lib.EpiParams(EPI_RESIDUAL, F32, _ptr(bias), None, 0, residual.data_ptr(), _stride(residual, "residual"))
         else:
             if out is None or out.shape != (M, N):
                 raise KernelError("gemm_mx: out must be [M, N]")
-            e = _lib.EpiParams(ACTIVATION_EPILOGUE[activation], dtype_code(out.dtype), _ptr(bias), out.data_ptr(), _rows(out, "out"))
+            e = _lib.EpiParams(ACTIVATION_EPILOGUE[activation], dtype_code(out.dtype), _ptr(bias), out.data_ptr(), _stride(out, "out"))
         e.exact = 1 if kind == _ROWS_F32 else 0
     if M == 0:
         return
