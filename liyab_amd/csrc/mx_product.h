@@ -29,8 +29,8 @@ __device__ __forceinline__ mx_bf16x8 mx_eight_of(uint32_t word, float power) {
     return mx_bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// mx_tiles.hip: products of many rows in bfloat16 or 8 bits, in tiles of 64 x 128, 128 x 128 or 256 x 256.
-enum : int { kMxTile128 = 1, kMxTile256 = 2, kMxTile64 = 3 };
+// mx_tiles.hip: products of many rows in bfloat16 or 8 bits, in tiles of 64 x 128, 128 x 128, 128 x 256 or 256 x 256.
+enum : int { kMxTile128 = 1, kMxTile256 = 2, kMxTile64 = 3, kMxTileWide = 4 };
 int launch_mx_tiles(int kind, int tile, const MxRowsIn& in, const uint8_t* blocks, int M, int N, int K, const EpiParams& epi, hipStream_t stream);
 
 }  // namespace liyab

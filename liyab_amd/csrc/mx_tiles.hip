@@ -12,7 +12,7 @@
 //             keeps 32 bits throughout.
 // What bounds it: the matrix instructions at 256 x 256 (2,048 x 16,384 x 4,096: bfloat16 186 us, 1,480 TFLOP/s; 8 bits 112 us, 2,440; 8,192 cubed 1,375 and
 // 2,525, where a library product of bfloat16 matrices reaches 1,359 and of e4m3 matrices 2,611); at the smaller tiles the instructions around them, of which a wave of 64 x 128
-// in 8 bits issues 70 a stage for its 8 products (2,048 x 4,096 x 4,096 at 128 x 128: 65 and 36 us; 512 rows at 64 x 128: 27 and 16). Measured on the way, us at 2,048 x
+// in 8 bits issues 70 a stage for its 8 products (2,048 x 4,096 x 4,096 at 128 x 256, one round of 256 workgroups: 58 and 34 us; 512 rows at 64 x 128: 27 and 16). Measured on the way, us at 2,048 x
 // 16,384 x 4,096 / 512 x 4,096 x 4,096 in 8 bits: loads' places worked out in each stage 119 / 21, kept in registers 116 / 17, the loads and the next stage's blocks spread
 // over the steps 112 / 17, the reads' places as constants of the instructions 112 / 15.7. Six stages in place of three change nothing.
 #include "common.h"
@@ -283,6 +283,7 @@ template <int ROWS>
 static int tile_of_size(int tile, const MxRowsIn& in, const uint8_t* blocks, int M, int N, int K, const EpiParams& epi, hipStream_t stream) {
     switch (tile) {
         case kMxTile64: return tile_of_epilogue<ROWS, 2, 2, 2, 4>(in, blocks, M, N, K, epi, stream);
+        case kMxTileWide: return tile_of_epilogue<ROWS, 2, 4, 4, 4>(in, blocks, M, N, K, epi, stream);
         case kMxTile128: return tile_of_epilogue<ROWS, 2, 2, 4, 4>(in, blocks, M, N, K, epi, stream);
         default: return tile_of_epilogue<ROWS, 2, 4, 8, 4>(in, blocks, M, N, K, epi, stream);
     }

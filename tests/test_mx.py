@@ -78,7 +78,7 @@ def test_the_products_waits_are_counted(source, tmp_path):
         assert spilled == 0 and scratch == 0, f"{k.split()[0]}: {spilled} registers spilled, {scratch} bytes of scratch a lane"
     if source == "mx_tiles.hip":
         tiles = re.findall(r"(?ms)^_ZN5liyab14mx_tile_kernel\S*:.*?^\.Lfunc_end", out.read_text())
-        assert len(tiles) == 54
+        assert len(tiles) == 72
         for t in tiles:
             # from the first product to the last; a stage's loads are the rows', the blocks' and one of scales
             loop = t[t.index("v_mfma"):t.rindex("v_mfma")]
