@@ -54,14 +54,38 @@ __device__ __forceinline__ void store_group(uint8_t* __restrict__ codes, uint8_t
 
 enum : int { kMxPlain = 0, kMxSilu = 1, kMxGeluTanh = 2, kMxClamped = 3 };
 
-// g / (1 + 2^t), the quotient mended by what it leaves over: of large values, where 1 + 2^t is 1, the reciprocal alone would be off by a step,
-// which moves some of them over a border of the 8-bit numbers (2,048 rows of 16,384: off by 1.3e-5 in the 2-norm without, no value moved with it).
-__device__ __forceinline__ float over_one_plus(float g, float t) {
-    const float d = 1.0f + __builtin_amdgcn_exp2f(t), rcp = __builtin_amdgcn_rcpf(d), q = g * rcp;
-    return d < 0x1p126f ? fmaf(fmaf(-q, d, g), rcp, q) : q;  // (beyond, the reciprocal is zero or has few bits)
+// Values next to a border of the 8-bit numbers, or of a group's scale, need more than 32 bits to fall on the right side: gates and norms are
+// computed in 64 (whose multiply-adds go at the rate of single 32-bit ones) and come to 32 rounded to odd, which no later rounding is misled by. In 32 bits
+// throughout some values of every 16 million landed on the wrong side, off by 1e-5 to 1e-4 in the 2-norm, now none (2,048 rows of 16,384: gates 54.5 us then,
+// 5.5 TB/s, and 56.0 now; norms of 2,048 rows of 4,096 19.7 and 20.4, 4.5 TB/s).
+__device__ __forceinline__ float to_odd(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = static_cast<uint32_t>(bits);
+    // 29 bits more than 32-bit numbers have: whether there is any becomes the last bit
+    const uint32_t cut = (lo | ((lo & 0x1fffffffu) + 0x1fffffffu)) & 0xe0000000u;
+    return static_cast<float>(__builtin_bit_cast(double, (bits & 0xffffffff00000000ull) | cut));
 }
-__device__ __forceinline__ float silu(float g) { return over_one_plus(g, -1.4426950408889634f * g); }
-__device__ __forceinline__ float gelu_tanh_of(float g) { return over_one_plus(g, (-2.0f * 0.7978845608028654f * 1.4426950408889634f) * fmaf(0.044715f * g * g, g, g)); }
+
+// g / (1 + 2^t). 2^r for |r| <= 1/2: the polynomial of degree 7 that meets it at the eight Chebyshev points, off by 6e-11 of it.
+__device__ __forceinline__ double over_one_plus(double g, double t) {
+    const double n = rint(t), r = t - n;
+    double e = 1.5303699899644103e-05;
+    e = fma(e, r, 0.00015469729234889767);
+    e = fma(e, r, 0.0013333478477891695);
+    e = fma(e, r, 0.009618025613220747);
+    e = fma(e, r, 0.05550410906319735);
+    e = fma(e, r, 0.240226512134995);
+    e = fma(e, r, 0.6931471805568348);
+    e = fma(e, r, 0.9999999999595616);
+    const double d = fmin(1.0 + __builtin_amdgcn_ldexp(e, static_cast<int>(n)), 1e300);  // (finite: an infinity's reciprocal could not be mended)
+    const double rcp = __builtin_amdgcn_rcp(d);
+    return g * fma(fma(-d, rcp, 1.0), rcp, rcp);
+}
+__device__ __forceinline__ double silu(double g) { return over_one_plus(g, -1.44269504088896340736 * g); }
+__device__ __forceinline__ double gelu_tanh_of(double g) {
+    constexpr double kSlope = -2.0 * 0.79788456080286535588 * 1.44269504088896340736;
+    return over_one_plus(g, g * fma(kSlope * 0.044715, g * g, kSlope));
+}
 
 template <typename T, int OP, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads)
@@ -78,11 +102,11 @@ mx_rows_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ s
         load8<WIDE>(u, p + d, i, d);
 #pragma unroll
         for (int j = 0; j < kLaneValues; ++j) {
-            if constexpr (OP == kMxSilu) v[j] = silu(v[j]) * u[j];
-            else if constexpr (OP == kMxGeluTanh) v[j] = gelu_tanh_of(v[j]) * u[j];
+            if constexpr (OP == kMxSilu) v[j] = to_odd(silu(v[j]) * u[j]);
+            else if constexpr (OP == kMxGeluTanh) v[j] = to_odd(gelu_tanh_of(v[j]) * u[j]);
             else {
                 const float g = fminf(v[j], limit);
-                v[j] = over_one_plus(g, -1.4426950408889634f * slope * g) * (fminf(fmaxf(u[j], -limit), limit) + shift);
+                v[j] = to_odd(over_one_plus(g, -1.44269504088896340736 * slope * g) * (static_cast<double>(fminf(fmaxf(u[j], -limit), limit)) + shift));
             }
             if (i + j >= d) v[j] = 0.0f;  // (behind the row)
         }
@@ -90,19 +114,59 @@ mx_rows_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ s
     store_group(codes + row * ldo, scales + row * lds, i, v);
 }
 
-// The sum over a workgroup of WAVES waves, the same bits in every lane.
+template <int CTRL>
+__device__ __forceinline__ double double_dpp(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits), CTRL, 0xf, 0xf, false), hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(bits >> 32), CTRL, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+__device__ __forceinline__ double double_of(double v, int lane) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(bits), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(bits >> 32), lane);
+    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
+}
+
+// The sum over a workgroup of WAVES waves, the same bits in every lane (the steps of `wave_sum`).
 template <int WAVES>
-__device__ __forceinline__ float group_total(float v, float* red) {
-    v = wave_sum(v);
+__device__ __forceinline__ double group_total(double v, double* red) {
+    v += double_dpp<0xB1>(v);
+    v += double_dpp<0x4E>(v);
+    v += double_dpp<0x141>(v);
+    v += double_dpp<0x140>(v);
+    v = (double_of(v, 0) + double_of(v, 16)) + (double_of(v, 32) + double_of(v, 48));
     if constexpr (WAVES > 1) {
         __syncthreads();
         if (threadIdx.x % kWave == 0) red[threadIdx.x / kWave] = v;
         __syncthreads();
-        v = 0.0f;
+        v = 0.0;
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) v += red[w];
     }
     return v;
+}
+
+// v scale weight + bias of eight neighbours, in 8 bits.
+template <bool WIDE>
+__device__ __forceinline__ void store_normed(uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, double (&v)[kLaneValues], double scale, const float* __restrict__ weight,
+                                             const float* __restrict__ bias, int i, int d) {
+    float w[kLaneValues], b[kLaneValues] = {}, y[kLaneValues];
+    if (weight != nullptr) {
+        load8<WIDE>(w, weight, i, d);
+#pragma unroll
+        for (int j = 0; j < kLaneValues; ++j) v[j] *= scale * w[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < kLaneValues; ++j) v[j] *= scale;
+    }
+    if (bias != nullptr) load8<WIDE>(b, bias, i, d);
+#pragma unroll
+    for (int j = 0; j < kLaneValues; ++j) y[j] = to_odd(v[j] + b[j]);
+    if (i + kLaneValues > d) {  // (a row of infinities has NaN behind its end too)
+#pragma unroll
+        for (int j = 0; j < kLaneValues; ++j)
+            if (i + j >= d) y[j] = 0.0f;
+    }
+    store_group(codes, scales, i, y);
 }
 
 // A row a workgroup, held in registers: TRIPS stretches of 8 values a lane.
@@ -110,21 +174,18 @@ template <int WAVES, int TRIPS, typename AddT, bool WIDE>
 __global__ void __launch_bounds__(WAVES * kWave)
 mx_norm_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const float* __restrict__ x, const AddT* __restrict__ add,
                float* __restrict__ stream, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int centred, int d) {
-    __shared__ float red[WAVES];
+    __shared__ double red[WAVES];
     constexpr int STEP = WAVES * kWave * kLaneValues;
     const int64_t row = blockIdx.x;
     const int i0 = threadIdx.x * kLaneValues;
-    float v[TRIPS][kLaneValues];
-    float sum = 0.0f;
+    double v[TRIPS][kLaneValues], sum = 0.0;
 #pragma unroll
     for (int t = 0; t < TRIPS; ++t) {
-        load8<WIDE>(v[t], x + row * d, i0 + t * STEP, d);
-        if (add != nullptr) {
-            float y[kLaneValues];
-            load8<WIDE>(y, add + row * d, i0 + t * STEP, d);
+        float a[kLaneValues], y[kLaneValues] = {};
+        load8<WIDE>(a, x + row * d, i0 + t * STEP, d);
+        if (add != nullptr) load8<WIDE>(y, add + row * d, i0 + t * STEP, d);
 #pragma unroll
-            for (int j = 0; j < kLaneValues; ++j) v[t][j] += y[j];
-        }
+        for (int j = 0; j < kLaneValues; ++j) v[t][j] = static_cast<double>(a[j]) + y[j];
     }
     if (stream != nullptr) {
         float* const s = stream + row * d;
@@ -132,56 +193,84 @@ mx_norm_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ s
         for (int t = 0; t < TRIPS; ++t) {
             const int i = i0 + t * STEP;
             if (WIDE && i + kLaneValues <= d) {
-                *reinterpret_cast<float4*>(s + i) = make_float4(v[t][0], v[t][1], v[t][2], v[t][3]);
-                *reinterpret_cast<float4*>(s + i + 4) = make_float4(v[t][4], v[t][5], v[t][6], v[t][7]);
+                *reinterpret_cast<float4*>(s + i) = make_float4(static_cast<float>(v[t][0]), static_cast<float>(v[t][1]), static_cast<float>(v[t][2]), static_cast<float>(v[t][3]));
+                *reinterpret_cast<float4*>(s + i + 4) = make_float4(static_cast<float>(v[t][4]), static_cast<float>(v[t][5]), static_cast<float>(v[t][6]), static_cast<float>(v[t][7]));
             } else {
 #pragma unroll
                 for (int j = 0; j < kLaneValues; ++j)
-                    if (i + j < d) s[i + j] = v[t][j];
+                    if (i + j < d) s[i + j] = static_cast<float>(v[t][j]);
             }
         }
     }
-    float mean = 0.0f;
+    double mean = 0.0;
     if (centred) {
 #pragma unroll
         for (int t = 0; t < TRIPS; ++t)
 #pragma unroll
             for (int j = 0; j < kLaneValues; ++j) sum += v[t][j];
-        mean = group_total<WAVES>(sum, red) / static_cast<float>(d);
-        sum = 0.0f;
+        mean = group_total<WAVES>(sum, red) / d;
+        sum = 0.0;
     }
 #pragma unroll
     for (int t = 0; t < TRIPS; ++t)
 #pragma unroll
         for (int j = 0; j < kLaneValues; ++j) {
-            v[t][j] = i0 + t * STEP + j < d ? v[t][j] - mean : 0.0f;
+            v[t][j] = i0 + t * STEP + j < d ? v[t][j] - mean : 0.0;
             sum += v[t][j] * v[t][j];
         }
-    const float scale = 1.0f / sqrtf(group_total<WAVES>(sum, red) / static_cast<float>(d) + eps);
+    const double scale = 1.0 / sqrt(group_total<WAVES>(sum, red) / d + eps);
 #pragma unroll
     for (int t = 0; t < TRIPS; ++t) {
         const int i = i0 + t * STEP;
         if (i >= ldo) continue;
-        float w[kLaneValues], b[kLaneValues];
-        if (weight != nullptr) {
-            load8<WIDE>(w, weight, i, d);
+        store_normed<WIDE>(codes + row * ldo, scales + row * lds, v[t], scale, weight, bias, i, d);
+    }
+}
+
+// Rows that registers do not hold: read again for the squares and for the result (from the stream, where it is written, which may be x).
+template <int WAVES, typename AddT, bool WIDE>
+__global__ void __launch_bounds__(WAVES * kWave)
+mx_norm_long_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const float* x, const AddT* add, float* stream,
+                    const float* __restrict__ weight, const float* __restrict__ bias, float eps, int centred, int d) {
+    __shared__ double red[WAVES];
+    constexpr int STEP = WAVES * kWave * kLaneValues;
+    const int64_t row = blockIdx.x;
+    const int i0 = threadIdx.x * kLaneValues;
+    const float* from = x + row * d;
+    const AddT* more = add == nullptr ? nullptr : add + row * d;
+    auto values = [&](double (&v)[kLaneValues], int i) {
+        float a[kLaneValues], y[kLaneValues] = {};
+        load8<WIDE>(a, from, i, d);
+        if (more != nullptr) load8<WIDE>(y, more, i, d);
 #pragma unroll
-            for (int j = 0; j < kLaneValues; ++j) v[t][j] = v[t][j] * scale * w[j];
-        } else {
+        for (int j = 0; j < kLaneValues; ++j) v[j] = static_cast<double>(a[j]) + y[j];
+    };
+    double v[kLaneValues], sum = 0.0, mean = 0.0;
+    for (int i = i0; i < d; i += STEP) {
+        values(v, i);
 #pragma unroll
-            for (int j = 0; j < kLaneValues; ++j) v[t][j] *= scale;
+        for (int j = 0; j < kLaneValues; ++j) {
+            if (stream != nullptr && i + j < d) stream[row * d + i + j] = static_cast<float>(v[j]);
+            sum += v[j];
         }
-        if (bias != nullptr) {
-            load8<WIDE>(b, bias, i, d);
+    }
+    if (stream != nullptr) from = stream + row * d, more = nullptr;
+    if (centred) mean = group_total<WAVES>(sum, red) / d;
+    sum = 0.0;
+    for (int i = i0; i < d; i += STEP) {
+        values(v, i);
 #pragma unroll
-            for (int j = 0; j < kLaneValues; ++j) v[t][j] += b[j];
+        for (int j = 0; j < kLaneValues; ++j) {
+            const double c = i + j < d ? v[j] - mean : 0.0;
+            sum += c * c;
         }
-        if (i + kLaneValues > d) {  // (a row of infinities has NaN behind its end too)
+    }
+    const double scale = 1.0 / sqrt(group_total<WAVES>(sum, red) / d + eps);
+    for (int i = i0; i < ldo; i += STEP) {
+        values(v, i);
 #pragma unroll
-            for (int j = 0; j < kLaneValues; ++j)
-                if (i + j >= d) v[t][j] = 0.0f;
-        }
-        store_group(codes + row * ldo, scales + row * lds, i, v[t]);
+        for (int j = 0; j < kLaneValues; ++j) v[j] -= mean;
+        store_normed<WIDE>(codes + row * ldo, scales + row * lds, v, scale, weight, bias, i, d);
     }
 }
 
@@ -246,7 +335,10 @@ static int norm_of_width(const NormArgs& a, bool wide) {
     if (a.d <= 4096) return launch_norm<4, 2, AddT>(a, wide);
     if (a.d <= 8192) return launch_norm<8, 2, AddT>(a, wide);
     if (a.d <= 16384) return launch_norm<16, 2, AddT>(a, wide);
-    return launch_norm<16, 8, AddT>(a, wide);
+    auto* kernel = wide ? &mx_norm_long_kernel<16, AddT, true> : &mx_norm_long_kernel<16, AddT, false>;
+    kernel<<<a.n, 16 * kWave, 0, a.stream>>>(static_cast<uint8_t*>(a.codes), a.ldo, static_cast<uint8_t*>(a.scales), a.lds, a.x, static_cast<const AddT*>(a.add),
+                                             a.stream_out, a.weight, a.bias, a.eps, a.centred, a.d);
+    return check_launch("mx_norm");
 }
 
 }  // namespace liyab
