@@ -119,7 +119,8 @@ class Mxfp4Matrix:
 
 class Mxfp8Rows:
     """Rows [n, width] in 8 bits: `codes` uint8 [n, width rounded up to 128] (e4m3, zeros behind the width) and `scales` uint8 [n, a byte a
-    group of 32, padded to 16]. `empty` and `pack` make the tensors; a workspace's may be given."""
+    group of 32, padded to 16]. `empty` and `pack` make the tensors; a workspace's may be given. The operators that write rows write all of a last chunk of 128:
+    who fills them otherwise leaves zeros behind the width in both (a byte of 255 there would make products of the row no numbers)."""
 
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, width: int):
         self.codes, self.scales, self.n, self.width = codes, scales, codes.shape[0], width
