@@ -1,9 +1,8 @@
 // Microscaling formats: 32 neighbours along a row share a power of two.
 //
 // A group of 32 values is 32 small floating-point numbers times 2^(s - 127), s a byte (255: the group is no number). Rows of
-// activations hold e4m3 numbers (8 bits, up to 448), matrices e2m1 numbers (4 bits: 0, 0.5, 1, 1.5, 2, 3, 4, 6). These are the
-// operands of gfx950's scaled matrix instruction (v_mfma_scale_f32_16x16x128_f8f6f4: 128 k, a scale a lane), and its conversions
-// (v_cvt_scalef32_pk_bf16_fp4, _f32_fp4) give two numbers with their scale an instruction, exactly: e2m1 times a power of two is a
+// activations hold e4m3 numbers (8 bits, up to 448), matrices e2m1 numbers (4 bits: 0, 0.5, 1, 1.5, 2, 3, 4, 6). gfx950's conversions
+// (v_cvt_scalef32_pk_bf16_fp4, _bf16_fp8, _f32_fp4) give two of them with their scale an instruction, exactly: a few bits times a power of two are a
 // bfloat16.
 //
 // The group's power of two follows from its largest magnitude alone, amax = m 2^x with 1 <= m < 2: s - 127 = x - emax, one more
@@ -27,8 +26,6 @@ constexpr int kMxStrip = 16;         // rows of a block
 constexpr int kMxBlockBytes = 1088;  // 64 lanes x 16 bytes, then 64 scales
 constexpr int kE4m3Max = 8, kE2m1Max = 2;  // exponents of the largest numbers
 
-typedef __attribute__((ext_vector_type(4))) int mx_i32x4;
-typedef __attribute__((ext_vector_type(8))) int mx_i32x8;
 typedef __attribute__((ext_vector_type(2))) float mx_f32x2;
 typedef __attribute__((ext_vector_type(2))) __bf16 mx_bf16x2;
 

@@ -29,6 +29,13 @@ __device__ __forceinline__ mx_bf16x8 mx_eight_of(uint32_t word, float power) {
     return mx_bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
+// Eight numbers of a row in 8 bits as bfloat16, scale and all: three bits of mantissa and a power of two, exact.
+__device__ __forceinline__ mx_bf16x8 mx_eight_of_rows(uint32_t lo, uint32_t hi, float power) {
+    const mx_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, true),
+                    c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, true);
+    return mx_bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
 // mx_tiles.hip: products of many rows in bfloat16 or 8 bits, in tiles of 64 x 128, 128 x 128, 128 x 256 or 256 x 256.
 enum : int { kMxTile128 = 1, kMxTile256 = 2, kMxTile64 = 3, kMxTileWide = 4 };
 int launch_mx_tiles(int kind, int tile, const MxRowsIn& in, const uint8_t* blocks, int M, int N, int K, const EpiParams& epi, hipStream_t stream);

@@ -8,9 +8,7 @@
 // of rows and matrix are in flight while the UNROLL before them, by then in registers, are multiplied; no wave waits for another until the end.
 //   bfloat16  two numbers a conversion, the group's scale with them, exact; four 16x16x32 instructions
 //   float32   the same in 32 bits; 32 16x16x4 instructions: chains of fused multiply-adds in 32 bits
-//   8 bits    the rows' numbers become bfloat16 too (three bits of mantissa and a power of two: exact), then as above. The scaled instruction
-//             takes them as they are, but adds eight neighbouring products without the bits that lie 14 places below the largest: sums
-//             of 32 bits, as here, cost nothing where memory sets the pace
+//   8 bits    the rows' numbers become bfloat16 too (three bits of mantissa and a power of two: exact), then as above
 // Chunk c of K goes to wave c % waves; the waves' sums meet in LDS in the waves' order.
 #include "common.h"
 #include "epilogue.h"
@@ -47,10 +45,7 @@ struct MxRowPart {
         } else {
             const uint4 p = piece[j / 2];
             const uint32_t lo = j % 2 == 0 ? p.x : p.z, hi = j % 2 == 0 ? p.y : p.w;
-            const float power = mx_power(scale);
-            const mx_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, true),
-                            c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, true);
-            return mx_bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+            return mx_eight_of_rows(lo, hi, mx_power(scale));
         }
     }
 };
@@ -242,8 +237,8 @@ enum : int { kShape1x1 = 11, kShape1x2 = 12, kShape2x1 = 21, kShape2x2 = 22, kSh
 // The shape that takes the least time: `fixed` and another `round` for each round of 256 workgroups, in us at 4,096 k (bfloat16 / 8-bit rows; measured over
 // matrices that are not in the caches, 24 to 2,048 rows of 768 to 16,384 columns; K changes them all much alike). The shapes of this file fill a compute unit
 // each; the smaller tiles leave room for others, so their rounds run into each other. What it chooses between, us: 512 rows 4,096 x 4,096 4x4 / 64 x 128
-// / 128 x 128 bfloat16 32 / 27 / 38, 8 bits 30 / 16 / 22; 2,048 rows 4,096 x 4,096 64 x 128 / 128 x 128 / 128 x 256 / 256 x 256 bfloat16 73 / 63 / 58 / 87, 8 bits 42 / 38 / 34 / 53,
-// 16,384 x 4,096 258 / 232 / 222 / 190, 147 / 133 / 127 / 112; 64 rows 4,096 x 4,096 2x1 / 4x1 / 2x4 12.8 / 10.6 / 10.8, 128 rows 2x1 / 2x4 / 4x4 22.8 / 10.6 / 16.4. Up to 16 rows the matrix's
+// / 128 x 128 bfloat16 32 / 29 / 38, 8 bits 30 / 25 / 38; 2,048 rows 4,096 x 4,096 64 x 128 / 128 x 128 / 128 x 256 / 256 x 256 bfloat16 72 / 64 / 59 / 87, 8 bits 67 / 59 / 58 / 91,
+// 16,384 x 4,096 264 / 237 / 228 / 198, 250 / 227 / 222 / 199; 64 rows 4,096 x 4,096 2x1 / 4x1 / 2x4 12.8 / 10.6 / 10.8, 128 rows 2x1 / 2x4 / 4x4 22.8 / 10.6 / 16.4. Up to 16 rows the matrix's
 // bytes set the pace: 16 waves a strip while every strip has a compute unit of its own (us, 16 waves / 8 waves on two strips: 1 row 1,600 x 6,400 5.0 / 6.7, 8
 // rows 4,096 x 4,096 5.3 / 6.3, 1 row 4,096 x 16,384 9.7 / 13.6), two strips beyond (1 row 16,384 x 4,096 12.4 / 10.1, 8 rows 6,400 x 1,600 6.2 / 4.5).
 // `same_bits`: eight waves whatever the rows, so that a row's sums have one order.
@@ -257,8 +252,8 @@ static int choose_shape(int kind, bool same_bits, int M, int N) {
     static const Shape shapes[] = {
         {kShape2x1, 32, 16, {0, 0}, {7.6f, 7.0f}},       {kShape2x2, 32, 32, {0, 0}, {9.0f, 8.5f}},        {kShape4x1, 64, 16, {0, 0}, {9.7f, 9.7f}},
         {kShape2x4, 32, 64, {0, 0}, {10.6f, 11.0f}},     {kShape4x2, 64, 32, {0, 0}, {12.1f, 12.4f}},      {kShape4x4, 64, 64, {0, 0}, {16.4f, 16.8f}},
-        {kMxTile64, 64, 128, {12.0f, 7.0f}, {15.3f, 8.7f}}, {kMxTile128, 128, 128, {10.5f, 7.0f}, {27.3f, 15.6f}}, {kMxTileWide, 128, 256, {0, 3}, {55.5f, 31.0f}},
-        {kMxTile256, 256, 256, {0, 0}, {92.0f, 56.0f}},
+        {kMxTile64, 64, 128, {12.0f, 10.0f}, {15.3f, 13.9f}}, {kMxTile128, 128, 128, {10.5f, 12.0f}, {27.3f, 26.4f}}, {kMxTileWide, 128, 256, {0, 1.0f}, {55.5f, 55.3f}},
+        {kMxTile256, 256, 256, {0, 0}, {92.0f, 95.0f}},
     };
     int best = kShape4x4;
     float least = 3e38f;

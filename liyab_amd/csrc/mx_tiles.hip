@@ -5,16 +5,15 @@
 // flight. Blocks lie in LDS as in memory, which is the order of the matrix instructions' operands; of a row the 16-byte piece p sits at position p ^ (row / 2 % 8), so that
 // 16 lanes' reads of 16 rows at one piece fall into different banks.
 //   bfloat16  a block's numbers become bfloat16 with their scale, two an instruction (exact), and meet 16x16x32 instructions
-//   8 bits    one scaled 16x16x128 instruction a block takes both operands and both scales as they are, at twice bfloat16's rate. It adds eight
-//             neighbouring products in a sum of their own, in which the bits below 2^-13 of the largest are cut off (measured: 2^-14 of it is lost,
-//             2^-13 is not), and those sums in 32 bits: the result is off by 5e-6 in the 2-norm, a four-hundredth of a rounding to
-//             bfloat16 and a five-thousandth of what rows in 8 bits are off from wider ones by. Up to 64 rows, where memory sets the pace, mx_product.hip
-//             keeps 32 bits throughout.
-// What bounds it: the matrix instructions at 256 x 256 (2,048 x 16,384 x 4,096: bfloat16 186 us, 1,480 TFLOP/s; 8 bits 112 us, 2,440; 8,192 cubed 1,375 and
-// 2,525, where a library product of bfloat16 matrices reaches 1,359 and of e4m3 matrices 2,611); at the smaller tiles the instructions around them, of which a wave of 64 x 128
-// in 8 bits issues 70 a stage for its 8 products (2,048 x 4,096 x 4,096 at 128 x 256, one round of 256 workgroups: 58 and 34 us; 512 rows at 64 x 128: 27 and 16). Measured on the way, us at 2,048 x
-// 16,384 x 4,096 / 512 x 4,096 x 4,096 in 8 bits: loads' places worked out in each stage 119 / 21, kept in registers 116 / 17, the loads and the next stage's blocks spread
-// over the steps 112 / 17, the reads' places as constants of the instructions 112 / 15.7. Six stages in place of three change nothing.
+//   8 bits    the rows' numbers become bfloat16 too on their way from LDS (three bits of mantissa and a power of two: exact), then as above: sums of 32
+//             bits, as wide rows have them. The scaled instruction (v_mfma_scale_f32_16x16x128_f8f6f4) would take both operands as they are at twice the rate, but it adds
+//             eight neighbouring products in a sum of their own, in which the bits below 2^-13 of the largest are cut off (measured: 2^-14 of it is lost, 2^-13 is not):
+//             5e-6 in the 2-norm over normal values, and all of what is left where large neighbours cancel. It took 118 us where this takes 199 (2,048 x 16,384 x 4,096).
+// What bounds it: the matrix instructions at 256 x 256 (2,048 x 16,384 x 4,096, no activation: 198 us with rows in bfloat16, 1,390 TFLOP/s, and 199 in 8 bits; 8,192 cubed 1,430 TFLOP/s
+// both, where a library product of bfloat16 matrices reaches 1,359); at the smaller tiles the instructions around them (2,048 x 4,096 x 4,096 at 128 x 256, one round of
+// 256 workgroups: 59 and 58 us; 512 rows at 64 x 128: 29 and 25, the narrower rows being half the bytes). Measured on the way, us at 2,048 x
+// 16,384 x 4,096 / 512 x 4,096 x 4,096 with the scaled instruction: loads' places worked out in each stage 119 / 21, kept in registers 116 / 17, the loads and the next stage's
+// blocks spread over the steps 112 / 17, the reads' places as constants of the instructions 112 / 15.7. Six stages in place of three change nothing.
 #include "common.h"
 #include "gemm_tile.h"
 #include "launchers.h"
@@ -116,45 +115,45 @@ mx_tile_kernel(MxRowsIn in, const uint8_t* __restrict__ blocks, int M, int N, in
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    // A stage is STEPS steps of TN products; a step's row operand comes from LDS AHEAD steps before it, also across stages: AHEAD steps before a stage's
-    // end everyone waits until the next one has arrived and this one has been read, and the loads of the third stage from here take its place.
+    // A stage is PHASES runs through the tile's rows, TM steps of TN products each; a phase multiplies eight of every lane's k. A step's row operand comes from
+    // LDS AHEAD steps before it, also across stages: AHEAD steps before a stage's end everyone waits until the next one has arrived and this one has been read,
+    // and the loads of the third stage from here take its place.
     // (Vectors of the compiler's own throughout: its reads of structs from LDS wait for every load into LDS.)
-    constexpr int STEPS = TM * (MX ? 1 : 2), AHEAD = MX ? 2 : 4;
+    constexpr int PHASES = MX ? 4 : 2, STEPS = TM * PHASES, AHEAD = 4;
     static_assert(STEPS % AHEAD == 0, "the operands' places are constants");
     struct Operand {
-        u32x4 lo, hi;    // (hi and scale: rows in 8 bits)
-        uint32_t scale;  // a chunk's four
+        u32x4 wide;      // eight k of bfloat16
+        u32x2 codes;     // or of 8 bits
+        uint32_t scale;  // and their group's byte
     };
     Operand ring[AHEAD];
     // (what a lane adds to a stage's place: everything else is a constant of the instruction)
     const int place = (r >> 1) & 7;  // (a tile's rows start at a multiple of 16)
-    const int row_lane = (wm * TM * 16 + r) * kStageBytes, piece0 = row_lane + ((MX ? g : 2 * g) ^ place) * 16, piece1 = row_lane + ((MX ? 4 + g : 2 * g + 1) ^ place) * 16;
-    const int row_scale_lane = Stage::ROW_SCALES_AT + (wm * TM * 16 + r) * 4;
+    const int row_lane = (wm * TM * 16 + r) * kStageBytes, piece0 = row_lane + ((2 * g) ^ place) * 16, piece1 = row_lane + ((2 * g + 1) ^ place) * 16;
+    const int row_scale_lane = Stage::ROW_SCALES_AT + (wm * TM * 16 + r) * 4 + g;
     const int code_lane = Stage::CODES_AT + wn * TN * Stage::BLOCK + (MX ? 16 * lane : (16 * (g / 2) + r) * 16 + g % 2 * 8);
     const int scale_lane = Stage::SCALES_AT + wn * TN * Stage::SCALES + (MX ? lane : 16 * (g / 2) + r);
     auto read = [&](Operand& x, const uint8_t* stage, int q) {
         const int i = q % TM, k = q / TM;
         if constexpr (MX) {
-            x.lo = *reinterpret_cast<const u32x4*>(stage + piece0 + i * 16 * kStageBytes);
-            x.hi = *reinterpret_cast<const u32x4*>(stage + piece1 + i * 16 * kStageBytes);
-            x.scale = *reinterpret_cast<const uint32_t*>(stage + row_scale_lane + i * 16 * 4);
+            x.codes = *reinterpret_cast<const u32x2*>(stage + (k < 2 ? piece0 : piece1) + k % 2 * 8 + i * 16 * kStageBytes);
+            x.scale = stage[row_scale_lane + i * 16 * 4];
         } else {
-            x.lo = *reinterpret_cast<const u32x4*>(stage + (k == 0 ? piece0 : piece1) + i * 16 * kStageBytes);
+            x.wide = *reinterpret_cast<const u32x4*>(stage + (k == 0 ? piece0 : piece1) + i * 16 * kStageBytes);
         }
     };
-    // A stage's blocks: of a lane's matrix rows 32 k (8 bits), or 16 k of the half, in bfloat16, where lane group g takes k 16 g .. 16 g + 15 of the 64.
+    // A stage's blocks: of a lane's matrix rows 32 k (8 bits: lane group g takes k 32 g .. 32 g + 31 of the 128), or 16 k of the half (bfloat16: k 16 g .. 16 g + 15 of the 64).
+    using Codes = std::conditional_t<MX, u32x4, u32x2>;
     struct Blocks {
-        u32x4 codes[MX ? TN : 1];
-        u32x2 half[MX ? 1 : TN];
+        Codes codes[TN];
         uint32_t scale[TN];
     };
     auto read_block = [&](Blocks& b, const uint8_t* stage, int j) {
-        if constexpr (MX) b.codes[j] = *reinterpret_cast<const u32x4*>(stage + code_lane + j * Stage::BLOCK);
-        else b.half[j] = *reinterpret_cast<const u32x2*>(stage + code_lane + j * Stage::BLOCK);
+        b.codes[j] = *reinterpret_cast<const Codes*>(stage + code_lane + j * Stage::BLOCK);
         b.scale[j] = stage[scale_lane + j * Stage::SCALES];
     };
-    // (bfloat16) eight k of the blocks as operands: those that are multiplied now, and those of the next eight
-    mx_bf16x8 w[MX ? 1 : TN], w_next[MX ? 1 : TN];
+    // eight k of the blocks as operands: those that are multiplied now, and those of the next phase
+    mx_bf16x8 w[TN], w_next[TN];
     Blocks now, next;
 
     uint8_t *here = lds, *after = lds + Stage::BYTES;
@@ -167,41 +166,31 @@ mx_tile_kernel(MxRowsIn in, const uint8_t* __restrict__ blocks, int M, int N, in
     for (int j = 0; j < TN; ++j) read_block(now, here, j);
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) read(ring[q], here, q);
-    if constexpr (!MX) {
 #pragma unroll
-        for (int j = 0; j < TN; ++j) w[j] = mx_eight_of(now.half[j][0], mx_power(now.scale[j]));
-    }
+    for (int j = 0; j < TN; ++j) w[j] = mx_eight_of(now.codes[j][0], mx_power(now.scale[j]));
     auto multiply = [&](Blocks& now, Blocks& next, int s) {
 #pragma unroll
         for (int j = 0; j < TN; ++j) asm volatile("" : "+v"(now.scale[j]));  // (whole registers: bytes, they would be made so, and waited for, in the stage before)
         in_turn(std::make_integer_sequence<int, STEPS>{}, [&](auto at) {
             constexpr int q = decltype(at)::value, i = q % TM, k = q / TM;
             Operand& x = ring[q % AHEAD];
-            if constexpr (MX) {
-                const mx_i32x8 rows8 = __builtin_shufflevector(__builtin_bit_cast(mx_i32x4, x.lo), __builtin_bit_cast(mx_i32x4, x.hi), 0, 1, 2, 3, 4, 5, 6, 7);
-                const uint32_t row_scale = x.scale >> (8 * g);
+            mx_bf16x8 rows8;
+            if constexpr (MX) rows8 = mx_eight_of_rows(x.codes[0], x.codes[1], mx_power(x.scale));
+            else rows8 = __builtin_bit_cast(mx_bf16x8, x.wide);
 #pragma unroll
-                for (int j = 0; j < TN; ++j) {
-                    const mx_i32x4 four = __builtin_bit_cast(mx_i32x4, now.codes[j]);  // (e2m1 operands are four registers)
-                    const mx_i32x8 w8 = __builtin_shufflevector(four, four, 0, 1, 2, 3, -1, -1, -1, -1);
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w8, rows8, acc[i][j], 4, 0, 0, now.scale[j], 0, row_scale);
-                }
-            } else {
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j], rows8, acc[i][j], 0, 0, 0);
+            if constexpr (k < PHASES - 1) {
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[j], __builtin_bit_cast(mx_bf16x8, x.lo), acc[i][j], 0, 0, 0);
-                if constexpr (k == 0) {
+                for (int j = 0; j < TN; ++j)
+                    if (j * TM / TN == i) w_next[j] = mx_eight_of(now.codes[j][k + 1], mx_power(now.scale[j]));
+            } else if constexpr (q >= STEPS - 2) {
 #pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        if (j * TM / TN == i) w_next[j] = mx_eight_of(now.half[j][1], mx_power(now.scale[j]));
-                } else if constexpr (q >= STEPS - 2) {
+                for (int j = 0; j < TN; ++j)
+                    if (j / (TN / 2) == q - (STEPS - 2)) w_next[j] = mx_eight_of(next.codes[j][0], mx_power(next.scale[j]));
+            }
+            if constexpr (i == TM - 1) {
 #pragma unroll
-                    for (int j = 0; j < TN; ++j)
-                        if (j / (TN / 2) == q - (STEPS - 2)) w_next[j] = mx_eight_of(next.half[j][0], mx_power(next.scale[j]));
-                }
-                if constexpr (i == TM - 1) {
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) w[j] = w_next[j];
-                }
+                for (int j = 0; j < TN; ++j) w[j] = w_next[j];
             }
             if constexpr (q == STEPS - AHEAD) {  // (behind the step's products, which hide the wait for the last reads)
 #pragma unroll

@@ -4,7 +4,7 @@ A group of 32 neighbours along a row shares a power of two, kept as one byte s: 
 holds e2m1 numbers (`Mxfp4Matrix`, a little over a quarter of bfloat16's bytes), rows of activations e4m3 numbers (`Mxfp8Rows`). The
 group's byte follows from its largest magnitude m 2^x, 1 <= m < 2: s - 127 = x - emax + (m > 1.75), emax = 2 and 8; numbers are rounded to
 nearest, ties to even. A group that holds an infinity or a NaN is NaN throughout. The reference serves 4-bit weights in formats of its own
-(src/core/quant.cpp, groups of 32 with a 16-bit scale); these are the ones that gfx950's matrix instructions read.
+(src/core/quant.cpp, groups of 32 with a 16-bit scale); these are the ones that gfx950's instructions convert and multiply.
 
     w = Mxfp4Matrix.quantize(weight)                 # once, at load
     gemm_mx(x, w, bias, out=y)                       # x bfloat16, float32 or Mxfp8Rows
@@ -269,8 +269,7 @@ def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[to
             activation: str = "none", kv=None, shape: int = 0) -> None:
     """out = act(a . w^T + bias), or residual += a . w^T + bias, or the paged query, key and value product (`kv` as `ops.gemm` takes it). a [M, K]: bfloat16 or
     float32 with contiguous rows, or `Mxfp8Rows`; out [M, N] bfloat16 or float32, residual float32. Products are exact in 32 bits
-    and their sums are 32-bit; where 8-bit rows are many, eight neighbouring products are added to 14 bits below their largest first (csrc/mx_tiles.hip). A row has the same
-    bits whatever the other rows if it is float32, or under `ops.batch_invariant`. `shape`: the workgroups' (csrc/mx_product.hip; 0: chosen from the sizes)."""
+    and their sums are 32-bit, whatever the rows' kind and number. A row has the same bits whatever the other rows if it is float32, or under `ops.batch_invariant`. `shape`: the workgroups' (csrc/mx_product.hip; 0: chosen from the sizes)."""
     index, K, N = w.index, w.width, w.rows
     if type(a) is Mxfp8Rows:
         kind, operand, M, dtype = _ROWS_MX, a.codes, a.n, torch.bfloat16

@@ -551,3 +551,34 @@ def test_a_gated_feed_forward_in_a_graph_and_on_another_stream(mx, n):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(x, expected)
+
+
+# -- sums ---------------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("shape", [0, 1, 2, 3, 4, 44])
+@pytest.mark.parametrize("M,N,K", [(65, 40, 128), (130, 257, 392), (300, 512, 1000)])
+def test_rows_in_8_bits_sum_in_32_bits(mx, M, N, K, shape):
+    """Eight neighbours of every row hold two that cancel beside six that lie up to 2^-15 below them, and the result is those six and the row's others. Their products are whole
+    multiples of 2^-8 and no partial sum reaches 2^13: 32 bits hold all of them, and nothing is off. Random rows are off by less than 2^-24 sqrt(K) in the 2-norm: a rounding
+    of 2^-25 of the sum in the mean at each of fewer than K additions that do not know of each other."""
+    rng = np.random.default_rng(M)
+    codes = np.zeros((M, K), dtype=np.uint8)
+    low = 8 + np.arange(1, 33)  # 2^-6 to 2^-2
+    codes[:] = rng.choice(low, size=(M, K)) | (128 * rng.integers(0, 2, size=(M, K))).astype(np.uint8)
+    at = rng.integers(0, K // 8, size=M) * 8
+    codes[np.arange(M), at], codes[np.arange(M), at + 1] = 126, 126 | 128  # 448 and -448
+    scales = np.full((M, -(-K // 32)), 127, dtype=np.uint8)
+    wc = np.repeat(7 | (8 * rng.integers(0, 2, size=(N, -(-K // 8)))), 8, axis=1)[:, :K].astype(np.uint8)  # 6 or -6, eight of a sign
+    ws = np.full((N, -(-K // 32)), 127, dtype=np.uint8)
+    w = mx.Mxfp4Matrix.pack(torch.from_numpy(plain_mx.two_a_byte(wc)).to(DEV), torch.from_numpy(ws).to(DEV), K)
+    a = mx.Mxfp8Rows.pack(torch.from_numpy(codes).to(DEV), torch.from_numpy(scales).to(DEV))
+    av, wv = plain_mx.values(codes, scales, plain_mx.E4M3), plain_mx.values(wc, ws, plain_mx.E2M1)
+    out = torch.empty(M, N, device=DEV)
+    mx.gemm_mx(a, w, None, out=out, shape=shape)
+    assert np.array_equal(out.double().cpu().numpy(), av @ wv.T)
+    w, wv = matrix(mx, N, K)
+    a, av = rows_of(mx, M, K, "mxfp8")
+    mx.gemm_mx(a, w, None, out=out, shape=shape)
+    want = av @ wv.T
+    assert np.linalg.norm(out.double().cpu().numpy() - want) < 2.0 ** -24 * K ** 0.5 * np.linalg.norm(want)
