@@ -21,7 +21,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 
 // Eight neighbours p[i .. i + 8), zeros from d on. WIDE: every row starts on a 16-byte boundary.
 template <bool WIDE, typename T>
-__device__ __forceinline__ void load8(float (&v)[kLaneValues], const T* __restrict__ p, int i, int d) {
+__device__ __forceinline__ void load8(float (&v)[kLaneValues], const T* p, int i, int d) {
     if (WIDE && i + kLaneValues <= d) {
         if constexpr (sizeof(T) == 4) {
             const float4 a = *reinterpret_cast<const float4*>(p + i), b = *reinterpret_cast<const float4*>(p + i + 4);
@@ -169,11 +169,11 @@ __device__ __forceinline__ void store_normed(uint8_t* __restrict__ codes, uint8_
     store_group(codes, scales, i, y);
 }
 
-// A row a workgroup, held in registers: TRIPS stretches of 8 values a lane.
+// A row a workgroup, held in registers: TRIPS stretches of 8 values a lane. The stream may be x: a lane loads all that it stores before it stores.
 template <int WAVES, int TRIPS, typename AddT, bool WIDE>
 __global__ void __launch_bounds__(WAVES * kWave)
-mx_norm_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const float* __restrict__ x, const AddT* __restrict__ add,
-               float* __restrict__ stream, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int centred, int d) {
+mx_norm_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const float* x, const AddT* add,
+               float* stream, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int centred, int d) {
     __shared__ double red[WAVES];
     constexpr int STEP = WAVES * kWave * kLaneValues;
     const int64_t row = blockIdx.x;

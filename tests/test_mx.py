@@ -87,3 +87,25 @@ def test_the_products_waits_are_counted(source, tmp_path):
             mx_rows, wm, wn, tm, tn = int(stage[1]) == 2, *(int(stage[i]) for i in range(2, 6))
             loads = wm * tm * 16 // 8 // (wm * wn) + wn * tn * (1024 if mx_rows else 512) // 1024 // (wm * wn) + 1
             assert counts == {loads}, f"{t.split(':')[0]}: waits until {sorted(counts)} loads are left, a stage has {loads}"
+
+
+def kernel_parameters(source, kernel, tmp_path):
+    """The parameters of every instantiation of a kernel, as the compiler's intermediate form declares them."""
+    hipcc = build.hipcc_path()
+    if hipcc is None:
+        pytest.skip("hipcc was not found")
+    out = tmp_path / "kernels.ll"
+    r = subprocess.run([hipcc, *build.FLAGS, *build.FILE_FLAGS.get(source, []), "-I", build.CSRC, "--cuda-device-only", "-emit-llvm", "-S", os.path.join(build.CSRC, source), "-o", str(out)],
+                       capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stderr[-2000:]
+    found = re.findall(rf"(?m)^define [^@]*amdgpu_kernel void @_ZN5liyab\d+{kernel}I[^(]*\((.*)\) local_unnamed_addr", out.read_text())
+    assert found
+    return [re.split(r", (?=ptr|i\d|float|double)", f) for f in found]
+
+
+@pytest.mark.parametrize("kernel", ["mx_norm_kernel", "mx_norm_long_kernel"])
+def test_the_norms_stream_may_be_their_input(kernel, tmp_path):
+    """`norm_mx` takes stream=x: the compiler is told nothing that the call breaks. (codes and scales are nobody else's: there it is told.)"""
+    for p in kernel_parameters("mx_rows.hip", kernel, tmp_path):
+        assert "noalias" in p[0] and "noalias" in p[2]
+        assert not any("noalias" in p[i] for i in (4, 5, 6)), f"{kernel}: x, add or stream are declared to be nobody else's: {p[4:7]}"
