@@ -227,7 +227,8 @@ mx_norm_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ s
     }
 }
 
-// Rows that registers do not hold: read again for the squares and for the result (from the stream, where it is written, which may be x).
+// Rows that registers do not hold: read again for the squares and for the result, each time as x + add, whose 64 bits the stream does not have. The stream
+// may be x: it is written with the result, by the lane that reads there.
 template <int WAVES, typename AddT, bool WIDE>
 __global__ void __launch_bounds__(WAVES * kWave)
 mx_norm_long_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const float* x, const AddT* add, float* stream,
@@ -236,26 +237,22 @@ mx_norm_long_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restric
     constexpr int STEP = WAVES * kWave * kLaneValues;
     const int64_t row = blockIdx.x;
     const int i0 = threadIdx.x * kLaneValues;
-    const float* from = x + row * d;
-    const AddT* more = add == nullptr ? nullptr : add + row * d;
     auto values = [&](double (&v)[kLaneValues], int i) {
         float a[kLaneValues], y[kLaneValues] = {};
-        load8<WIDE>(a, from, i, d);
-        if (more != nullptr) load8<WIDE>(y, more, i, d);
+        load8<WIDE>(a, x + row * d, i, d);
+        if (add != nullptr) load8<WIDE>(y, add + row * d, i, d);
 #pragma unroll
         for (int j = 0; j < kLaneValues; ++j) v[j] = static_cast<double>(a[j]) + y[j];
     };
     double v[kLaneValues], sum = 0.0, mean = 0.0;
-    for (int i = i0; i < d; i += STEP) {
-        values(v, i);
+    if (centred) {
+        for (int i = i0; i < d; i += STEP) {
+            values(v, i);
 #pragma unroll
-        for (int j = 0; j < kLaneValues; ++j) {
-            if (stream != nullptr && i + j < d) stream[row * d + i + j] = static_cast<float>(v[j]);
-            sum += v[j];
+            for (int j = 0; j < kLaneValues; ++j) sum += v[j];
         }
+        mean = group_total<WAVES>(sum, red) / d;
     }
-    if (stream != nullptr) from = stream + row * d, more = nullptr;
-    if (centred) mean = group_total<WAVES>(sum, red) / d;
     sum = 0.0;
     for (int i = i0; i < d; i += STEP) {
         values(v, i);
@@ -269,7 +266,10 @@ mx_norm_long_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restric
     for (int i = i0; i < ldo; i += STEP) {
         values(v, i);
 #pragma unroll
-        for (int j = 0; j < kLaneValues; ++j) v[j] -= mean;
+        for (int j = 0; j < kLaneValues; ++j) {
+            if (stream != nullptr && i + j < d) stream[row * d + i + j] = static_cast<float>(v[j]);
+            v[j] -= mean;
+        }
         store_normed<WIDE>(codes + row * ldo, scales + row * lds, v, scale, weight, bias, i, d);
     }
 }

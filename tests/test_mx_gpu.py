@@ -582,3 +582,31 @@ def test_rows_in_8_bits_sum_in_32_bits(mx, M, N, K, shape):
     mx.gemm_mx(a, w, None, out=out, shape=shape)
     want = av @ wv.T
     assert np.linalg.norm(out.double().cpu().numpy() - want) < 2.0 ** -24 * K ** 0.5 * np.linalg.norm(want)
+
+
+def beside_borders(c, seed):
+    """Weights that put c / rms(c) of a row next to borders of e4m3, as near as 32 bits can say them (a few 2^-26 of a value); 400, and with it the groups' scale, in every 32nd place."""
+    rng = np.random.default_rng(seed)
+    d = c.size
+    v = (8 + rng.integers(0, 8, size=d) + 0.5) * np.exp2(rng.integers(-3, 8, size=d) - 3.0)
+    v[::32] = 400.0
+    return (v / (np.abs(c) / np.sqrt((c ** 2).mean()))).astype(np.float32)
+
+
+@pytest.mark.parametrize("centred", [False, True])
+@pytest.mark.parametrize("to", ["nowhere", "beside", "x"])
+@pytest.mark.parametrize("d", [1600, 16384, 20000])
+def test_norms_next_to_borders_whatever_the_width_and_the_stream(mx, d, to, centred):
+    """x + add is not rounded ahead of the norm, whether the stream is written or not, and where: a rounding to 32 bits would move values by up to 2^-24 of them across borders that lie nearer.
+    In 64 bits both sides are off by some 1e-15: one of these values in 10^7 lies that close."""
+    x, add = rnd(1, d, seed=31), rnd(1, d, seed=32)
+    t = x.double().cpu().numpy() + add.double().cpu().numpy()
+    c = t - t.mean() if centred else t
+    w = torch.from_numpy(beside_borders(c[0], 33)).to(DEV)
+    out = empty_rows(mx, 1, d)
+    stream = {"nowhere": None, "beside": torch.empty_like(x), "x": x}[to]
+    want = x + add
+    mx.norm_mx(out, x, w, 0.0, centred=centred, add=add, stream=stream)
+    y = c / np.sqrt((c ** 2).mean()) * w.double().cpu().numpy()
+    check_rows(out, *plain_mx.quantize(y, plain_mx.E4M3, 8), to)
+    assert stream is None or torch.equal(stream, want)
