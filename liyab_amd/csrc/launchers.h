@@ -233,10 +233,10 @@ int liyab_mx_pack(void* blocks, const void* codes, int64_t ldc, const void* scal
 int liyab_mx_dense(void* w, int dtype, int64_t ldw, const void* blocks, int N, int K, hipStream_t stream);
 int liyab_mx_align(void* out, int ldo, const void* in, int64_t ldi, int size, int n, int d, hipStream_t stream);
 int liyab_mx_rows(void* codes, int64_t ldo, void* scales, int64_t lds, const void* x, int dtype, int64_t ldx, int n, int d, hipStream_t stream);
-int liyab_mx_glu(void* codes, int64_t ldo, void* scales, int64_t lds, const float* gu, int64_t ld, int n, int d, int act, float limit, float slope,
-                 float shift, hipStream_t stream);
+int liyab_mx_glu(void* codes, int64_t ldo, void* scales, int64_t lds, const float* gu, int64_t ld, int n, int d, int act, double limit, double slope,
+                 double shift, hipStream_t stream);
 int liyab_mx_norm(void* codes, int64_t ldo, void* scales, int64_t lds, const float* x, const void* add, int add_dtype, float* stream_out,
-                  const float* weight, const float* bias, float eps, int centred, int n, int d, hipStream_t stream);
+                  const float* weight, const float* bias, double eps, int centred, int n, int d, hipStream_t stream);
 int liyab_mx_product(const void* a, int64_t lda, const void* a_scales, int64_t lds, int rows, const void* blocks, int M, int N, int K,
                      int tile, const liyab::EpiParams* epi, hipStream_t stream);
 }  // extern "C"

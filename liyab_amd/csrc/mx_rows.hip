@@ -90,7 +90,7 @@ __device__ __forceinline__ double gelu_tanh_of(double g) {
 template <typename T, int OP, bool WIDE>
 __global__ void __launch_bounds__(kRowThreads)
 mx_rows_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const T* __restrict__ in, int64_t ldi, int d, int blocks_a_row,
-               float limit, float slope, float shift) {
+               double limit, double slope, double shift) {
     const int64_t row = blockIdx.x / blocks_a_row;
     const int i = (blockIdx.x % blocks_a_row * kRowThreads + threadIdx.x) * kLaneValues;
     if (i >= ldo) return;  // (whole quads: rows of codes are whole chunks)
@@ -105,8 +105,8 @@ mx_rows_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ s
             if constexpr (OP == kMxSilu) v[j] = to_odd(silu(v[j]) * u[j]);
             else if constexpr (OP == kMxGeluTanh) v[j] = to_odd(gelu_tanh_of(v[j]) * u[j]);
             else {
-                const float g = fminf(v[j], limit);
-                v[j] = to_odd(over_one_plus(g, -1.44269504088896340736 * slope * g) * (static_cast<double>(fminf(fmaxf(u[j], -limit), limit)) + shift));
+                const double g = fmin(v[j], limit);
+                v[j] = to_odd(over_one_plus(g, -1.44269504088896340736 * slope * g) * (fmin(fmax(u[j], -limit), limit) + shift));
             }
             if (i + j >= d) v[j] = 0.0f;  // (behind the row)
         }
@@ -173,7 +173,7 @@ __device__ __forceinline__ void store_normed(uint8_t* __restrict__ codes, uint8_
 template <int WAVES, int TRIPS, typename AddT, bool WIDE>
 __global__ void __launch_bounds__(WAVES * kWave)
 mx_norm_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const float* x, const AddT* add,
-               float* stream, const float* __restrict__ weight, const float* __restrict__ bias, float eps, int centred, int d) {
+               float* stream, const float* __restrict__ weight, const float* __restrict__ bias, double eps, int centred, int d) {
     __shared__ double red[WAVES];
     constexpr int STEP = WAVES * kWave * kLaneValues;
     const int64_t row = blockIdx.x;
@@ -232,7 +232,7 @@ mx_norm_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ s
 template <int WAVES, typename AddT, bool WIDE>
 __global__ void __launch_bounds__(WAVES * kWave)
 mx_norm_long_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ scales, int64_t lds, const float* x, const AddT* add, float* stream,
-                    const float* __restrict__ weight, const float* __restrict__ bias, float eps, int centred, int d) {
+                    const float* __restrict__ weight, const float* __restrict__ bias, double eps, int centred, int d) {
     __shared__ double red[WAVES];
     constexpr int STEP = WAVES * kWave * kLaneValues;
     const int64_t row = blockIdx.x;
@@ -295,8 +295,8 @@ static int check_rows(const char* what, const void* codes, int64_t ldo, const vo
 }
 
 template <typename T, int OP>
-static int launch_rows(const char* what, void* codes, int64_t ldo, void* scales, int64_t lds, const void* in, int64_t ldi, int n, int d, float limit, float slope,
-                       float shift, hipStream_t stream) {
+static int launch_rows(const char* what, void* codes, int64_t ldo, void* scales, int64_t lds, const void* in, int64_t ldi, int n, int d, double limit, double slope,
+                       double shift, hipStream_t stream) {
     const int per_row = static_cast<int>((ldo / kLaneValues + kRowThreads - 1) / kRowThreads);
     const int64_t grid = static_cast<int64_t>(n) * per_row;
     LIYAB_REQUIRE(grid < (int64_t{1} << 31), "%s: %d rows of %d values are too many", what, n, d);
@@ -315,7 +315,7 @@ struct NormArgs {
     const void* add;
     float* stream_out;
     const float *weight, *bias;
-    float eps;
+    double eps;
     int centred, n, d;
     hipStream_t stream;
 };
@@ -355,11 +355,11 @@ extern "C" int liyab_mx_rows(void* codes, int64_t ldo, void* scales, int64_t lds
 }
 
 // act 0: silu, 1: the tanh form of gelu, 2: clamped halves (limit, slope, shift).
-extern "C" int liyab_mx_glu(void* codes, int64_t ldo, void* scales, int64_t lds, const float* gu, int64_t ld, int n, int d, int act, float limit, float slope,
-                            float shift, hipStream_t stream) {
+extern "C" int liyab_mx_glu(void* codes, int64_t ldo, void* scales, int64_t lds, const float* gu, int64_t ld, int n, int d, int act, double limit, double slope,
+                            double shift, hipStream_t stream) {
     if (const int rc = check_rows("mx_glu", codes, ldo, scales, lds, n, d)) return rc;
     LIYAB_REQUIRE(gu != nullptr && ld >= 2 * static_cast<int64_t>(d), "mx_glu: needs rows of 2 x %d values", d);
-    LIYAB_REQUIRE(act != 2 || limit > 0.0f, "mx_glu: the limit must be positive");
+    LIYAB_REQUIRE(act != 2 || limit > 0.0, "mx_glu: the limit must be positive");
     if (n == 0) return 0;
     if (act == 0) return launch_rows<float, kMxSilu>("mx_glu", codes, ldo, scales, lds, gu, ld, n, d, 0, 0, 0, stream);
     if (act == 1) return launch_rows<float, kMxGeluTanh>("mx_glu", codes, ldo, scales, lds, gu, ld, n, d, 0, 0, 0, stream);
@@ -368,7 +368,7 @@ extern "C" int liyab_mx_glu(void* codes, int64_t ldo, void* scales, int64_t lds,
 }
 
 extern "C" int liyab_mx_norm(void* codes, int64_t ldo, void* scales, int64_t lds, const float* x, const void* add, int add_dtype, float* stream_out,
-                             const float* weight, const float* bias, float eps, int centred, int n, int d, hipStream_t stream) {
+                             const float* weight, const float* bias, double eps, int centred, int n, int d, hipStream_t stream) {
     if (const int rc = check_rows("mx_norm", codes, ldo, scales, lds, n, d)) return rc;
     LIYAB_REQUIRE(x != nullptr && d <= 65536, "mx_norm: needs rows of up to 65,536 values, got %d", d);
     if (n == 0) return 0;

@@ -10,7 +10,7 @@
 //
 // A list is a sequence of records of 64-bit words:
 //   [launcher index, number of arguments, arguments ..., number of block words, block words ...]
-// An argument is the value's bits (integers sign-extended, a float's 32 bits in the low half).
+// An argument is the value's bits (integers sign-extended, a float's 32 bits in the low half, a double's 64).
 // The argument that points at the epilogue's parameter block holds kBlockArg instead; the block's
 // bytes follow the arguments, and the launcher gets their address.
 #include "launchers.h"
@@ -40,6 +40,14 @@ struct Arg<float> {
         float f;
         std::memcpy(&f, &lo, 4);
         return f;
+    }
+};
+template <>
+struct Arg<double> {
+    static double get(uint64_t bits) {
+        double d;
+        std::memcpy(&d, &bits, 8);
+        return d;
     }
 };
 

@@ -153,8 +153,8 @@ _SIGNATURES = {
     "liyab_mx_pack": [P, P, c_int64, P, c_int64, c_int, c_int, P],
     "liyab_mx_dense": [P, c_int, c_int64, P, c_int, c_int, P],
     "liyab_mx_rows": [P, c_int64, P, c_int64, P, c_int, c_int64, c_int, c_int, P],
-    "liyab_mx_glu": [P, c_int64, P, c_int64, P, c_int64, c_int, c_int, c_int, c_float, c_float, c_float, P],
-    "liyab_mx_norm": [P, c_int64, P, c_int64, P, P, c_int, P, P, P, c_float, c_int, c_int, c_int, P],
+    "liyab_mx_glu": [P, c_int64, P, c_int64, P, c_int64, c_int, c_int, c_int, c_double, c_double, c_double, P],
+    "liyab_mx_norm": [P, c_int64, P, c_int64, P, P, c_int, P, P, P, c_double, c_int, c_int, c_int, P],
     "liyab_mx_align": [P, c_int, P, c_int64, c_int, c_int, c_int, P],
     "liyab_mx_product": [P, c_int64, P, c_int64, c_int, P, c_int, c_int, c_int, c_int, _EPI_PTR, P],
 }
@@ -237,7 +237,7 @@ def _encoders(name: str):
         for t in _SIGNATURES[name]:
             kinds.append("block" if t is _EPI_PTR else "float" if t is c_float else "double" if t is c_double else
                          "address" if t is P else "int")
-        hit = _entries[name] = (index, kinds) if index >= 0 and n.value == len(kinds) and "double" not in kinds else (-1, kinds)
+        hit = _entries[name] = (index, kinds) if index >= 0 and n.value == len(kinds) else (-1, kinds)
     return hit
 
 
@@ -261,6 +261,8 @@ def _record(name: str, args) -> None:
             words.append((0 if a is None else int(a)) & _U64)
         elif kind == "float":
             words.append(struct.unpack("<I", struct.pack("<f", a))[0])
+        elif kind == "double":
+            words.append(struct.unpack("<Q", struct.pack("<d", a))[0])
         else:
             raw = bytes(a._obj)  # (the argument is ctypes.byref(params))
             raw += b"\0" * (-len(raw) % 8)

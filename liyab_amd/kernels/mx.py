@@ -218,7 +218,7 @@ def rows_mx(out: Mxfp8Rows, x: torch.Tensor) -> None:
 
 def glu_mx(out: Mxfp8Rows, gu: torch.Tensor, activation: str, clamp=None) -> None:
     """out = act(G) * U in 8 bits; gu float32 [n, 2 * d] = [G | U]; act "silu" or "gelu_tanh", or "clamped" with clamp = (limit, slope, shift): g *
-    sigmoid(slope * g) * (u + shift), g = min(G, limit), u = clamp(U, -limit, limit) (`ops.glu`, `ops.glu_clamped`). Computed in 64 bits, as `norm_mx`."""
+    sigmoid(slope * g) * (u + shift), g = min(G, limit), u = clamp(U, -limit, limit) (`ops.glu`, `ops.glu_clamped`). Computed in 64 bits, `clamp`'s numbers too, as `norm_mx`."""
     ld = _stride(gu, "gu")
     n, d2 = gu.shape
     if gu.dtype != torch.float32 or d2 != 2 * out.width:
@@ -241,7 +241,7 @@ def norm_mx(out: Mxfp8Rows, x: torch.Tensor, weight: Optional[torch.Tensor], eps
             add: Optional[torch.Tensor] = None, stream: Optional[torch.Tensor] = None) -> None:
     """With t = x + add: out = t / sqrt(mean(t^2) + eps) * weight (+ bias) in 8 bits; `centred`: a layer norm, (t - mean(t)) / sqrt(var(t) + eps) * weight
     + bias. x float32 [n, d], d up to 65,536; `add` [n, d] float32 or bfloat16 (a sublayer's result); `stream` float32 [n, d] gets t (it may be
-    x itself). Computed in 64 bits: values next to a border of the 8-bit numbers land on its right side."""
+    x itself). Computed in 64 bits, eps too: values next to a border of the 8-bit numbers land on its right side."""
     _dev(x, "x")
     if x.dtype != torch.float32 or x.dim() != 2 or not x.is_contiguous():
         raise KernelError(f"norm_mx: x must be contiguous float32 [n, d], got {tuple(x.shape)} {x.dtype}")

@@ -610,3 +610,38 @@ def test_norms_next_to_borders_whatever_the_width_and_the_stream(mx, d, to, cent
     y = c / np.sqrt((c ** 2).mean()) * w.double().cpu().numpy()
     check_rows(out, *plain_mx.quantize(y, plain_mx.E4M3, 8), to)
     assert stream is None or torch.equal(stream, want)
+
+
+def test_what_gates_and_norms_are_given_is_taken_in_64_bits(mx):
+    """A slope and a shift that 32 bits do not hold, and an eps as large as the squares, over values beside borders that the rounded numbers would put on the other side. Gates are off by
+    up to 6e-11 of a value: those that lie nearer than 1e-9 of it to a border are left out."""
+    rng = np.random.default_rng(41)
+    limit, slope, shift = 6.7, 1.702, 1.1
+
+    def gate(g, u, slope, shift):
+        g = np.minimum(g, limit)
+        return g / (1 + np.exp(-slope * g)) * (np.clip(u, -limit, limit) + shift)
+
+    def place(v):  # among the borders of numbers with three bits of mantissa
+        e = np.floor(np.log2(np.abs(v)))
+        return 8 * e + np.floor((np.abs(v) * np.exp2(-e) * 16 + 1) / 2)
+
+    g = rng.uniform(0.5, 3.0, size=1 << 14).astype(np.float32).astype(np.float64)
+    border = (8 + rng.integers(0, 8, size=g.size) + 0.5) * np.exp2(rng.integers(-2, 4, size=g.size) - 3.0)
+    u = (border / gate(g, 1.0 - shift, slope, shift) - shift).astype(np.float32).astype(np.float64)
+    y, low = gate(g, u, slope, shift), gate(g, u, float(np.float32(slope)), float(np.float32(shift)))
+    near = np.flatnonzero((np.abs(u) < 6) & (place(y) != place(low)) & (place(y * (1 - 1e-9)) == place(y * (1 + 1e-9))))
+    n = near.size // 31
+    assert n > 20
+    g, u = (np.concatenate([np.full((n, 1), b), v[near[:31 * n]].reshape(n, 31)], axis=1) for b, v in ((6.0, g), (9.0, u)))  # (6 and 9, a gate of 46.8: the groups' scale)
+    out = empty_rows(mx, n, 32)
+    mx.glu_mx(out, torch.from_numpy(np.concatenate([g, u], axis=1)).float().to(DEV), "clamped", clamp=(limit, slope, shift))
+    check_rows(out, *plain_mx.quantize(gate(g, u, slope, shift), plain_mx.E4M3, 8), "clamped")
+
+    x, eps = rnd(1, 4096, seed=42, scale=0.01), 1e-4
+    v = x.double().cpu().numpy()
+    c = v / np.sqrt((v ** 2).mean() + eps)
+    w = torch.from_numpy((beside_borders(v[0], 43).astype(np.float64) * (v / np.sqrt((v ** 2).mean()) / c)[0]).astype(np.float32)).to(DEV)
+    out = empty_rows(mx, 1, 4096)
+    mx.norm_mx(out, x, w, eps)
+    check_rows(out, *plain_mx.quantize(c * w.double().cpu().numpy(), plain_mx.E4M3, 8), "norm")
