@@ -105,8 +105,9 @@ mx_rows_kernel(uint8_t* __restrict__ codes, int64_t ldo, uint8_t* __restrict__ s
             if constexpr (OP == kMxSilu) v[j] = to_odd(silu(v[j]) * u[j]);
             else if constexpr (OP == kMxGeluTanh) v[j] = to_odd(gelu_tanh_of(v[j]) * u[j]);
             else {
-                const double g = fmin(v[j], limit);
-                v[j] = to_odd(over_one_plus(g, -1.44269504088896340736 * slope * g) * (fmin(fmax(u[j], -limit), limit) + shift));
+                // (comparisons, which leave NaN what it is)
+                const double g = v[j] > limit ? limit : v[j], c = u[j] > limit ? limit : u[j] < -limit ? -limit : u[j];
+                v[j] = to_odd(over_one_plus(g, -1.44269504088896340736 * slope * g) * (c + shift));
             }
             if (i + j >= d) v[j] = 0.0f;  // (behind the row)
         }

@@ -645,3 +645,31 @@ def test_what_gates_and_norms_are_given_is_taken_in_64_bits(mx):
     out = empty_rows(mx, 1, 4096)
     mx.norm_mx(out, x, w, eps)
     check_rows(out, *plain_mx.quantize(c * w.double().cpu().numpy(), plain_mx.E4M3, 8), "norm")
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh", "clamped"])
+def test_gates_of_what_is_no_number(mx, activation):
+    """A NaN in either half makes its group no number, and no other; an infinity does where nothing clamps it."""
+    d, clamp = 200, (2.5, 1.702, 1.0) if activation == "clamped" else None
+    gu = rnd(6, 2 * d, seed=51)
+    plain = empty_rows(mx, 6, d)
+    mx.glu_mx(plain, gu, activation, clamp=clamp)
+    gu[0, 40] = gu[1, d + 70] = gu[2, 199] = gu[2, 2 * d - 1] = float("nan")
+    gu[3, 33], gu[4, d + 33] = float("inf"), float("-inf")
+    out = empty_rows(mx, 6, d)
+    mx.glu_mx(out, gu, activation, clamp=clamp)
+    scales = out.scales.cpu().numpy()[:, :7]
+    no_number = np.zeros((6, 7), dtype=bool)
+    no_number[0, 1] = no_number[1, 2] = no_number[2, 6] = True
+    no_number[3, 1] = no_number[4, 1] = activation != "clamped"
+    assert np.array_equal(scales == 255, no_number)
+    same = ~np.repeat(no_number, 32, axis=1)[:, :d]
+    same[3:5, 32:64] = False
+    assert np.array_equal(out.codes.cpu().numpy()[:, :d][same], plain.codes.cpu().numpy()[:, :d][same])
+    if activation == "clamped":  # what lies beyond the limits is the limit
+        gu[3, 33], gu[4, d + 33] = 2.5, -2.5
+        for i in range(3):
+            gu[i] = 0.0
+        again = empty_rows(mx, 6, d)
+        mx.glu_mx(again, gu, activation, clamp=clamp)
+        assert torch.equal(again.codes[3:], out.codes[3:])
