@@ -54,8 +54,10 @@ glu_clamped_kernel(T* __restrict__ out, const float* __restrict__ gu, int64_t ld
     const int i = blockIdx.x * EW_THREADS + threadIdx.x;
     if (i >= ff) return;
     const float* row = gu + static_cast<int64_t>(t) * ld;
-    const float g = fminf(row[i], limit);
-    const float u = fminf(fmaxf(row[ff + i], -limit), limit);
+    // (comparisons, which leave NaN what it is)
+    const float g0 = row[i], u0 = row[ff + i];
+    const float g = g0 > limit ? limit : g0;
+    const float u = u0 > limit ? limit : u0 < -limit ? -limit : u0;
     const float scale = gate != nullptr ? logistic(gate[t * gate_stride]) : 1.0f;
     out[static_cast<int64_t>(t) * ff + i] = from_float<T>(g * logistic(slope * g) * (u + shift) * scale);
 }

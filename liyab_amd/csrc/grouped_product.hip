@@ -56,7 +56,7 @@ __device__ __forceinline__ float grouped_act(const GroupedParams& p, float v0, f
     float v = v0;
     if constexpr (NW == 2) {
         if (p.act == 2) {
-            const float g = fminf(v0, p.limit), u = fminf(fmaxf(v1, -p.limit), p.limit);
+            const float g = v0 > p.limit ? p.limit : v0, u = v1 > p.limit ? p.limit : v1 < -p.limit ? -p.limit : v1;  // (comparisons, which leave NaN what it is)
             v = g * gp_sigmoid(p.slope * g) * (u + p.shift);
         } else v = v0 * gp_sigmoid(v0) * v1;
     }
