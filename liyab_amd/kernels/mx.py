@@ -170,6 +170,8 @@ class Mxfp8Rows:
 
 
 def _check_out(out: Mxfp8Rows, n: int, d: int, what: str) -> None:
+    if not isinstance(out, Mxfp8Rows):
+        raise KernelError(f"{what}: the result goes to Mxfp8Rows, not to {type(out).__name__}")
     if out.n != n or out.width != d:
         raise KernelError(f"{what}: the rows have places for [{out.n}, {out.width}], not [{n}, {d}]")
 
@@ -221,8 +223,8 @@ def glu_mx(out: Mxfp8Rows, gu: torch.Tensor, activation: str, clamp=None) -> Non
     sigmoid(slope * g) * (u + shift), g = min(G, limit), u = clamp(U, -limit, limit) (`ops.glu`, `ops.glu_clamped`). Computed in 64 bits, `clamp`'s numbers too, as `norm_mx`."""
     ld = _stride(gu, "gu")
     n, d2 = gu.shape
-    if gu.dtype != torch.float32 or d2 != 2 * out.width:
-        raise KernelError(f"glu_mx: needs float32 [n, {2 * out.width}], got {tuple(gu.shape)} {gu.dtype}")
+    if gu.dtype != torch.float32 or d2 % 2:
+        raise KernelError(f"glu_mx: needs float32 [n, 2 * d], got {tuple(gu.shape)} {gu.dtype}")
     _check_out(out, n, d2 // 2, "glu_mx")
     stream = _on("glu_mx", out.index, gu)
     if (activation == "clamped") != (clamp is not None) or (clamp is None and activation not in GLU_ACTIVATIONS):
@@ -267,11 +269,19 @@ def norm_mx(out: Mxfp8Rows, x: torch.Tensor, weight: Optional[torch.Tensor], eps
 
 def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
             activation: str = "none", kv=None, shape: int = 0) -> None:
-    """out = act(a . w^T + bias), or residual += a . w^T + bias, or the paged query, key and value product (`kv` as `ops.gemm` takes it). a [M, K]: bfloat16 or
+    """out = act(a . w^T + bias), or residual += a . w^T + bias, or the paged query, key and value product (`kv` as `ops.gemm` takes it): one of the three. a [M, K]: bfloat16 or
     float32 with contiguous rows, or `Mxfp8Rows`; out [M, N] bfloat16 or float32, residual float32. Products are exact in 32 bits
-    and their sums are 32-bit, whatever the rows' kind and number. A row has the same bits whatever the other rows if it is float32, or under `ops.batch_invariant`. `shape`: the workgroups' (csrc/mx_product.hip; 0: chosen from the sizes)."""
+    and their sums are 32-bit, whatever the rows' kind and number. A row has the same bits whatever the other rows if it is float32, or under `ops.batch_invariant`. `shape`: the workgroups' (csrc/mx_product.hip; 0: chosen from the sizes), for bfloat16 and 8-bit rows."""
+    if not isinstance(w, Mxfp4Matrix):
+        raise KernelError(f"gemm_mx: the matrix is a Mxfp4Matrix, not {type(w).__name__}")
+    if residual is not None and (out is not None or kv is not None):
+        raise KernelError("gemm_mx: the result is added to a residual or goes to out, not both")
+    if activation != "none" and (residual is not None or kv is not None):
+        raise KernelError(f"gemm_mx: activation '{activation}' is for results that go to out")
+    if activation not in ACTIVATION_EPILOGUE:
+        raise KernelError(f"gemm_mx: activation '{activation}' is not known")
     index, K, N = w.index, w.width, w.rows
-    if type(a) is Mxfp8Rows:
+    if isinstance(a, Mxfp8Rows):
         kind, operand, M, dtype = _ROWS_MX, a.codes, a.n, torch.bfloat16
         if a.width != K:
             raise KernelError(f"gemm_mx: rows of {a.width} values, a matrix of width {K}")
@@ -282,6 +292,8 @@ def gemm_mx(a, w: Mxfp4Matrix, bias: Optional[torch.Tensor], *, out: Optional[to
         if width != K or (dtype is not torch.bfloat16 and dtype is not torch.float32):
             raise KernelError(f"gemm_mx: a {tuple(a.shape)} {dtype} does not fit a matrix of {N} x {K}")
         kind, per = (_ROWS_BF16, 8) if dtype is torch.bfloat16 else (_ROWS_F32, 4)
+        if shape and kind == _ROWS_F32:
+            raise KernelError(f"gemm_mx: float32 rows have one shape of workgroups, not shape {shape}")
     stream = _on("gemm_mx", index, operand, bias, out, residual, *(kv[:3] if kv is not None else ()))
     if kv is not None:
         e = _epilogue(_Like(M, dtype), w, bias, out, None, EPI_QKV_PAGED, kv)

@@ -673,3 +673,36 @@ def test_gates_of_what_is_no_number(mx, activation):
         again = empty_rows(mx, 6, d)
         mx.glu_mx(again, gu, activation, clamp=clamp)
         assert torch.equal(again.codes[3:], out.codes[3:])
+
+
+def test_calls_that_say_two_things_are_refused(mx):
+    """Nothing that a call says is left out in silence, and nothing of it is done where it is refused."""
+    from liyab_amd.errors import KernelError
+
+    w, _ = matrix(mx, 32, 64)
+    a, wide = rnd(4, 64, dtype=torch.bfloat16), rnd(4, 64)
+    out, stream, rows = torch.zeros(4, 32, device=DEV), torch.zeros(4, 32, device=DEV), mx.Mxfp8Rows.empty(4, 64)
+    kc = torch.zeros(2, 1, 16, 8, dtype=torch.bfloat16, device=DEV)
+    q, vc, slots = torch.zeros(4, 16, dtype=torch.bfloat16, device=DEV), kc.clone(), torch.arange(4, dtype=torch.int32, device=DEV)
+    bad = [
+        lambda: mx.gemm_mx(a, w, None, residual=stream, activation="gelu_tanh"),
+        lambda: mx.gemm_mx(a, w, None, residual=stream, out=out),
+        lambda: mx.gemm_mx(a, w, None, residual=stream, kv=(kc, vc, slots, 16)),
+        lambda: mx.gemm_mx(a, w, None, out=q, kv=(kc, vc, slots, 16), activation="gelu_erf"),
+        lambda: mx.gemm_mx(a, w, None, out=out, activation="relu"),
+        lambda: mx.gemm_mx(a, w, None, out=out, activation=None),
+        lambda: mx.gemm_mx(wide, w, None, out=out, shape=1),
+        lambda: mx.gemm_mx(a, w, None, out=out, shape=5),
+        lambda: mx.gemm_mx(a, rnd(32, 64, dtype=torch.bfloat16), None, out=out),
+        lambda: mx.rows_mx(out, wide),
+        lambda: mx.norm_mx(out, wide, None, 1e-5),
+        lambda: mx.glu_mx(out, rnd(4, 128), "silu"),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(KernelError):
+            call()
+            pytest.fail(f"call {i} was taken")
+    for t in (out, stream, q, kc, vc):
+        assert not t.any()
+    mx.gemm_mx(a, w, None, out=q, kv=(kc, vc, slots, 16))
+    assert q.any() and kc.any() and vc.any()
