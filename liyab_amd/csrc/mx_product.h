@@ -18,9 +18,10 @@ struct MxRowsIn {
     int64_t lds;
 };
 
-// What a load behind a row's end reads instead: zeros, so that the zeros of the matrix there meet numbers.
-static __device__ __constant__ const uint32_t kMxZeros[4] = {0, 0, 0, 0};
-__device__ __forceinline__ const uint32_t* mx_zeros() { return kMxZeros; }
+// What a load behind a row's end reads instead: zeros, so that the zeros of the matrix there meet numbers. (One value, aligned as loads of 16 bytes take it.)
+typedef __attribute__((ext_vector_type(4))) uint32_t mx_u32x4;
+static __device__ __constant__ const mx_u32x4 kMxZeros = {0, 0, 0, 0};
+__device__ __forceinline__ const mx_u32x4* mx_zeros() { return &kMxZeros; }
 
 // Eight numbers of a block's row as bfloat16, scale and all: exact.
 __device__ __forceinline__ mx_bf16x8 mx_eight_of(uint32_t word, float power) {

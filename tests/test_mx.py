@@ -109,3 +109,14 @@ def test_the_norms_stream_may_be_their_input(kernel, tmp_path):
     for p in kernel_parameters("mx_rows.hip", kernel, tmp_path):
         assert "noalias" in p[0] and "noalias" in p[2]
         assert not any("noalias" in p[i] for i in (4, 5, 6)), f"{kernel}: x, add or stream are declared to be nobody else's: {p[4:7]}"
+
+
+def test_what_loads_behind_a_row_read_is_aligned_as_they_read(tmp_path):
+    """Loads into LDS take 16 bytes: the zeros' own type says that they start on such a boundary."""
+    hipcc = build.hipcc_path()
+    if hipcc is None:
+        pytest.skip("hipcc was not found")
+    source = tmp_path / "zeros.hip"
+    source.write_text('#include "mx_product.h"\nusing namespace liyab;\nstatic_assert(alignof(decltype(*mx_zeros())) >= 16 && sizeof(*mx_zeros()) == 16, "a load\'s 16 bytes");\n')
+    r = subprocess.run([hipcc, *build.FLAGS, "-I", build.CSRC, "--cuda-device-only", "-fsyntax-only", str(source)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
