@@ -239,11 +239,19 @@ def glu_mx(out: Mxfp8Rows, gu: torch.Tensor, activation: str, clamp=None) -> Non
               float(limit), float(slope), float(shift), stream)
 
 
+def _shifted(t: torch.Tensor, other: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory other than value by value."""
+    a, b = t.data_ptr(), other.data_ptr()
+    if a == b and t.dtype == other.dtype:
+        return False
+    return a < b + other.numel() * other.element_size() and b < a + t.numel() * t.element_size()
+
+
 def norm_mx(out: Mxfp8Rows, x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, *, bias: Optional[torch.Tensor] = None, centred: bool = False,
             add: Optional[torch.Tensor] = None, stream: Optional[torch.Tensor] = None) -> None:
     """With t = x + add: out = t / sqrt(mean(t^2) + eps) * weight (+ bias) in 8 bits; `centred`: a layer norm, (t - mean(t)) / sqrt(var(t) + eps) * weight
     + bias. x float32 [n, d], d up to 65,536; `add` [n, d] float32 or bfloat16 (a sublayer's result); `stream` float32 [n, d] gets t (it may be
-    x itself). Computed in 64 bits, eps too: values next to a border of the 8-bit numbers land on its right side."""
+    x itself, or `add`, but lie across neither). Computed in 64 bits, eps too: values next to a border of the 8-bit numbers land on its right side."""
     _dev(x, "x")
     if x.dtype != torch.float32 or x.dim() != 2 or not x.is_contiguous():
         raise KernelError(f"norm_mx: x must be contiguous float32 [n, d], got {tuple(x.shape)} {x.dtype}")
@@ -261,6 +269,8 @@ def norm_mx(out: Mxfp8Rows, x: torch.Tensor, weight: Optional[torch.Tensor], eps
     if stream is not None and (stream.dtype != torch.float32 or stream.shape != x.shape or not stream.is_contiguous()):
         raise KernelError(f"norm_mx: the stream must be contiguous float32 [{n}, {d}], got {tuple(stream.shape)} {stream.dtype}")
     to = _on("norm_mx", out.index, x, weight, bias, add, stream)
+    if stream is not None and (_shifted(stream, x) or (add is not None and _shifted(stream, add))):
+        raise KernelError("norm_mx: the stream lies across what the norm reads")
     if n == 0:
         return
     _lib.call("liyab_mx_norm", out.codes.data_ptr(), out.codes.shape[1], out.scales.data_ptr(), out.scales.shape[1], x.data_ptr(), _ptr(add), code, _ptr(stream),

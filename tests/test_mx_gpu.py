@@ -706,3 +706,25 @@ def test_calls_that_say_two_things_are_refused(mx):
         assert not t.any()
     mx.gemm_mx(a, w, None, out=q, kv=(kc, vc, slots, 16))
     assert q.any() and kc.any() and vc.any()
+
+
+@pytest.mark.parametrize("d", [64, 300, 20000])
+def test_the_stream_is_what_the_norm_reads_or_lies_apart(mx, d):
+    """x and add may be the stream, value by value; a stream that lies across either of them would be read where another row has written."""
+    from liyab_amd.errors import KernelError
+
+    n, w = 3, 1 + 0.2 * rnd(d, seed=61)
+    x, add = rnd(n, d, seed=62), rnd(n, d, seed=63)
+    want, stream = mx.Mxfp8Rows.empty(n, d), torch.empty(n, d, device=DEV)
+    mx.norm_mx(want, x, w, 1e-5, add=add, stream=stream)
+    for which in ("x", "add"):
+        a, b, out = x.clone(), add.clone(), mx.Mxfp8Rows.empty(n, d)
+        mx.norm_mx(out, a, w, 1e-5, add=b, stream=a if which == "x" else b)
+        assert torch.equal(a if which == "x" else b, stream) and torch.equal(out.codes, want.codes) and torch.equal(out.scales[:, : d // 32], want.scales[:, : d // 32])
+    flat = torch.zeros((n + 1) * d, device=DEV)
+    low, high = flat[: n * d].view(n, d), flat[d:].view(n, d)
+    half = flat.view(torch.bfloat16)[: n * d].view(n, d)
+    for kw in (dict(x=low, stream=high), dict(x=high, stream=low), dict(x=x, add=low, stream=high), dict(x=x, add=half, stream=low)):
+        with pytest.raises(KernelError):
+            mx.norm_mx(want, kw.pop("x"), w, 1e-5, **kw)
+    assert not flat.any()
