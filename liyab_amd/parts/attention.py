@@ -134,9 +134,9 @@ class Attention:
         self.kv_dim = self.n_kv_head * self.head_dim
         qkv_out = self.q_dim + 2 * self.kv_dim
         t = spec.tensors
-        self.qkv_weight = product_matrix(store, store.fetch(t["qkv_weight"], (qkv_out, self.width), "matrix"))
+        self.qkv_weight = product_matrix(store, t["qkv_weight"], (qkv_out, self.width))
         self.qkv_bias = store.fetch(t["qkv_bias"], (qkv_out,), "vector") if "qkv_bias" in t else None
-        self.out_weight = product_matrix(store, store.fetch(t["out_weight"], (self.width, self.q_dim), "matrix"))
+        self.out_weight = product_matrix(store, t["out_weight"], (self.width, self.q_dim))
         self.out_bias = store.fetch(t["out_bias"], (self.width,), "vector") if "out_bias" in t else None
         pos = getattr(spec, "position", None)
         self.position = build_part("position", pos, store, dtype) if pos is not None else None

@@ -31,9 +31,9 @@ class DenseFFN:
         if self.activation not in ("gelu_tanh", "gelu_erf"):
             raise ValueError(f"unknown activation '{self.activation}'")
         t = spec.tensors
-        self.up_weight = product_matrix(store, store.fetch(t["up_weight"], (self.inner, self.width), "matrix"))
+        self.up_weight = product_matrix(store, t["up_weight"], (self.inner, self.width))
         self.up_bias = store.fetch(t["up_bias"], (self.inner,), "vector") if "up_bias" in t else None
-        self.down_weight = product_matrix(store, store.fetch(t["down_weight"], (self.width, self.inner), "matrix"))
+        self.down_weight = product_matrix(store, t["down_weight"], (self.width, self.inner))
         self.down_bias = store.fetch(t["down_bias"], (self.width,), "vector") if "down_bias" in t else None
 
     defers = True  # forward(..., defer=True) takes the stream split or whole and may hand it back split
@@ -74,8 +74,8 @@ class ClampedGLU:
         if not self.limit > 0:
             raise ValueError(f"clamped feed-forward: a limit of {self.limit}")
         t = spec.tensors
-        self.in_weight = product_matrix(store, store.fetch_joined([t["gate"], t["up"]], [(self.inner, self.width)] * 2, "matrix", "rows"))
-        self.down_weight = product_matrix(store, store.fetch(t["down"], (self.width, self.inner), "matrix"))
+        self.in_weight = product_matrix(store, [t["gate"], t["up"]], [(self.inner, self.width)] * 2)
+        self.down_weight = product_matrix(store, t["down"], (self.width, self.inner))
 
     def begin(self, h, ctx: StepContext) -> torch.Tensor:
         """The first product, [gate | up] of h in 32 bits: everything of the feed-forward that reads its input. A block whose
@@ -127,8 +127,8 @@ class GatedFFN:
         if self.activation not in ops.GLU_ACTIVATIONS:
             raise ValueError(f"gated feed-forward: activation '{self.activation}' is not known")
         t = spec.tensors
-        self.in_weight = product_matrix(store, store.fetch_joined([t["gate"], t["up"]], [(self.inner, self.width)] * 2, "matrix", "rows"))
-        self.down_weight = product_matrix(store, store.fetch(t["down"], (self.width, self.inner), "matrix"))
+        self.in_weight = product_matrix(store, [t["gate"], t["up"]], [(self.inner, self.width)] * 2)
+        self.down_weight = product_matrix(store, t["down"], (self.width, self.inner))
 
     def begin(self, h, ctx: StepContext) -> torch.Tensor:
         """The first product, [gate | up] of h in 32 bits: everything of the feed-forward that reads its input. In steps of few rows the
@@ -186,9 +186,9 @@ class NormedPowersFFN:
         if int(spec.powers) != 3:
             raise ValueError(f"a mix of {spec.powers} powers (3 are taken)")
         t = spec.tensors
-        self.up_weight = product_matrix(store, store.fetch(t["up"], (self.inner, self.width), "matrix"))
+        self.up_weight = product_matrix(store, t["up"], (self.inner, self.width))
         self.act = store.fetch(t["act"], (4,), "vector")
-        self.down_weight = product_matrix(store, store.fetch(t["down"], (self.width, self.inner), "matrix"))
+        self.down_weight = product_matrix(store, t["down"], (self.width, self.inner))
 
     def begin(self, h, ctx: StepContext) -> torch.Tensor:
         """The first product in 32 bits: everything of the feed-forward that reads its input."""

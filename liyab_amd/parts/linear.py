@@ -56,11 +56,26 @@ def _fuses_exactly(a, w: torch.Tensor, residual) -> bool:
     return ops.is_batch_invariant() and w.dtype == a.norm.dtype == torch.bfloat16 and ops.norm_in_rows_pays(a.n_rows, w.shape[0], a.norm.width)
 
 
-def product_matrix(store, w: torch.Tensor):
-    """What `linear` multiplies by: the matrix as the store keeps matrices for products, in 4 bits (`mx.Mxfp4Matrix`) where the model is served so. For
+def product_matrix(store, src, shape, layout=None):
+    """What `linear` multiplies by: the matrix [out, in] that `src` names (a list: their rows one after the other, `shape` a list too), or another layout of
+    it, `layout` = (a key that names it, a function of the matrix). Where the model is served so, in 4 bits (`mx.Mxfp4Matrix`), and the wide matrix is not kept. For
     matrices that only `linear` reads."""
-    keep = getattr(store, "for_products", None)
-    return w if keep is None else keep(w)
+    several = isinstance(src, list)
+    four_bits = getattr(store, "products", None) is not None
+
+    def wide():
+        if several:
+            w = store.fetch_joined(src, shape, "matrix", "rows", keep=not four_bits)
+        else:
+            w = store.fetch(src, shape, "matrix", keep=not four_bits)
+        if layout is None:
+            return w
+        return layout[1](w) if four_bits else store.derived(layout[0], lambda: layout[1](w))
+
+    if not four_bits:
+        return wide()
+    names = tuple((s.name, s.layout) + tuple(rows_columns) for s, rows_columns in zip(*((src, shape) if several else ([src], [shape]))))
+    return store.in_4_bits(names + (layout[0] if layout is not None else ()), wide)
 
 
 def eight_bits(w) -> bool:

@@ -121,7 +121,7 @@ class ScoredAttention:
             srcs.append(t["gate"])
             shapes.append((H * V, d))
             at += H * V
-        self.in_weight = product_matrix(store, store.fetch_joined(srcs, shapes, "matrix", "rows"))
+        self.in_weight = product_matrix(store, srcs, shapes)
         # biases on the projections of queries, keys and values: one vector over the joint product's columns, zeros for the gate's
         self.in_bias = None
         if getattr(spec, "biased", False):
@@ -143,16 +143,14 @@ class ScoredAttention:
         if self.value_mix not in ("", "first", "later") or (self.value_mix and self.values_are_keys):
             raise ValueError(f"scored attention: value_mix '{self.value_mix}'")
         self.v_lam = store.fetch(t["vmix"], (), "vector").reshape(1) if self.value_mix else None
-        self.out_weight = store.fetch(t["out"], (d, H * V), "matrix")
         # Keys and values of different widths: both planes of the pages as wide as the wider (a multiple of 8), zeros behind the
         # narrower heads, which is what the engine's paged attention kernels take; zeros in keys and queries add nothing to a
         # score, zeros in values give zeros in the result, and the output projection gets zero columns for them.
-        self.row_dim = 0
+        self.row_dim, layout = 0, None
         if D != V and not self.gated and max(D, V) <= ops.ATTENTION_MAX_HEAD_DIM:
             P = self.row_dim = -(-max(D, V) // 8) * 8
-            w = self.out_weight
-            self.out_weight = store.derived(("padded_heads", t["out"].name, P), lambda: torch.nn.functional.pad(w.view(d, H, V), (0, P - V)).reshape(d, H * P).contiguous())
-        self.out_weight = product_matrix(store, self.out_weight)
+            layout = (("padded_heads", t["out"].name, P), lambda w: torch.nn.functional.pad(w.view(d, H, V), (0, P - V)).reshape(d, H * P).contiguous())
+        self.out_weight = product_matrix(store, t["out"], (d, H * V), layout)
         per_q, per_k = (H * D, G * D) if self.norm_rows else (D, D)
         normed = spec.qk_norm or self.norm_rows
         if spec.qk_norm and not getattr(spec, "qk_norm_weights", True):

@@ -36,7 +36,7 @@ class SelectiveScan:
         if self.taps < 1:
             raise ValueError(f"selective scan: a convolution of {self.taps} taps")
         t = spec.tensors
-        self.in_weight = product_matrix(store, store.fetch(t["in"], (2 * W, d), "matrix"))
+        self.in_weight = product_matrix(store, t["in"], (2 * W, d))
         self.conv = store.fetch(t["conv"], (W, self.taps), "vector")
         self.conv_bias = store.fetch(t["conv_bias"], (W,), "vector")
         self.x_weight = store.fetch(t["x"], (R + 2 * N, W), "matrix")
@@ -50,7 +50,7 @@ class SelectiveScan:
         # [states, channels], times log2(e): a decay is 2^(dt a)
         self.a2 = store.derived(("decay_rates", t["A_log"].name), lambda: (a_log.double().exp() * -math.log2(math.e)).t().float().contiguous())
         self.skip = store.fetch(t["D"], (W,), "vector")
-        self.out_weight = product_matrix(store, store.fetch(t["out"], (d, W), "matrix"))
+        self.out_weight = product_matrix(store, t["out"], (d, W))
 
     @property
     def takes_mx_rows(self) -> bool:

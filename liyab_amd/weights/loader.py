@@ -11,7 +11,7 @@ Precision: matrices and tables go to the device in the compute dtype of the
 path (bfloat16 for serving, float32 for the 32-bit path); vectors (norm
 weights, biases) are float32 on both paths; integer tensors become int32.
 A tensor is converted once, at load, and stays resident. With `products="mxfp4"` the matrices that parts
-hand to products alone (`for_products`) are kept in 4 bits instead, rounded from the compute dtype's, and with
+hand to products alone (`in_4_bits`) are kept in 4 bits instead, rounded from the compute dtype's, and with
 `rows="mxfp8"` these products take their rows in 8 bits.
 """
 
@@ -52,7 +52,7 @@ class WeightStore:
         if rows is not None and compute_dtype == torch.float32:
             raise InvalidArgument("rows in 8 bits are for the bfloat16 path: the float32 path keeps its rows in 32 bits")
         self.products, self.rows = products, rows
-        self._in_4_bits: Dict[tuple, tuple] = {}
+        self._in_4_bits: Dict[tuple, object] = {}
         self._tensors = tensors
         self.device = torch.device(device)
         self.compute_dtype = compute_dtype
@@ -85,16 +85,18 @@ class WeightStore:
     def has(self, src: TensorSource) -> bool:
         return self._resolve(src.name) is not None
 
-    def fetch_joined(self, srcs: Sequence[TensorSource], shapes: Sequence[Sequence[int]], role: str, how: str = "rows") -> torch.Tensor:
+    def fetch_joined(self, srcs: Sequence[TensorSource], shapes: Sequence[Sequence[int]], role: str, how: str = "rows", keep: bool = True) -> torch.Tensor:
         """Several tensors of the file as one on the device: how = "rows", one after the other along their
         first axis (projections of one input that run as one product), or "stack", along a new first axis
         (the matrices of a layer's experts). The parts are not kept on their own; asked for again with the
-        same names, the same device tensor comes back (layers that share their weights share it)."""
+        same names, the same device tensor comes back (layers that share their weights share it; unless it is not to be kept)."""
         key = (how, role) + tuple((s.name, s.layout) for s in srcs)
         hit = self._derived.get(key)
         if hit is None:
             parts = [self.fetch(src, shape, role, keep=False) for src, shape in zip(srcs, shapes)]
-            hit = self._derived[key] = (torch.cat(parts, dim=0) if how == "rows" else torch.stack(parts, dim=0)).contiguous()
+            hit = (torch.cat(parts, dim=0) if how == "rows" else torch.stack(parts, dim=0)).contiguous()
+            if keep:
+                self._derived[key] = hit
         return hit
 
     def derived(self, key: tuple, make) -> torch.Tensor:
@@ -105,19 +107,16 @@ class WeightStore:
             hit = self._derived[key] = make()
         return hit
 
-    def for_products(self, w: torch.Tensor):
-        """The matrix w [out, in] as products read it: itself, or in 4 bits. The same matrix gives the same object (layers that share their weights share it)."""
-        if self.products is None:
-            return w
+    def in_4_bits(self, key: tuple, make):
+        """The matrix [out, in] that `make` gives, in 4 bits, kept under `key` (which names what it was made of) so that layers sharing their weights share it. The wide
+        one is let go: a model takes the device's memory in 4 bits, and one wide matrix at a time."""
         from ..kernels.mx import Mxfp4Matrix
 
-        key = (w.data_ptr(), tuple(w.shape))
         hit = self._in_4_bits.get(key)
         if hit is None:
-            m = Mxfp4Matrix.quantize(w)
-            m.eight_bit_rows = self.rows is not None
-            hit = self._in_4_bits[key] = (w, m)  # (with w: its address stays its own)
-        return hit[1]
+            hit = self._in_4_bits[key] = Mxfp4Matrix.quantize(make())
+            hit.eight_bit_rows = self.rows is not None
+        return hit
 
     def fetch(self, src: TensorSource, shape: Sequence[int], role: str, keep: bool = True) -> Optional[torch.Tensor]:
         """The tensor `src` names, on the device, in working layout and dtype.

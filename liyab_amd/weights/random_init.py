@@ -76,7 +76,7 @@ class DrawingStore:
             raise ValueError(f"random weights: '{src.name}' is asked for as {list(stored)} and as {list(t.shape)}")
         return t.t() if src.layout == "in_out" else t
 
-    def fetch_joined(self, srcs, shapes, role: str, how: str = "rows") -> torch.Tensor:
+    def fetch_joined(self, srcs, shapes, role: str, how: str = "rows", keep: bool = True) -> torch.Tensor:
         parts = [self.fetch(src, shape, role) for src, shape in zip(srcs, shapes)]
         return torch.cat(parts, dim=0) if how == "rows" else torch.stack(parts, dim=0)
 

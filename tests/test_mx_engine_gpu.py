@@ -253,3 +253,43 @@ def test_generation_and_the_command_line(model_dirs):
                        capture_output=True, text=True, timeout=100)
     assert r.returncode == 0, r.stderr[-2000:]
     assert [int(t) for t in r.stdout.replace(",", " ").split()] == want
+
+
+def test_loading_holds_one_wide_matrix_at_a_time(tmp_path):
+    """A model that fits the device's memory in 4 bits loads there: what is allocated on the way stays under the 4-bit model, the tables and one matrix, as it is stored (4 bytes) and as
+    it is rounded (2, and 2 more where it is stored the other way round)."""
+    from liyab_amd.models.loading import load_model
+    from liyab_amd.weights import write_random_model
+
+    width, layers, vocab = 512, 6, 64
+    config = dict(CONFIG_A, n_layer=layers, n_embd=width, n_head=8, vocab_size=vocab, n_positions=128)
+    write_random_model(str(tmp_path), config, 5)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    _, model = load_model(str(tmp_path), "bfloat16", "cuda:0", weights="mxfp4")
+    values = 12 * width * width * layers
+    peak = torch.cuda.max_memory_allocated() - before
+    assert peak < values * 17 // 32 + 4 * width * width * 8 + (vocab + 128) * width * 8 + (1 << 20), f"{peak} bytes on the way, the wide matrices are {2 * values}"
+    one, other = model.blocks[0].ffn, model.blocks[1].ffn
+    assert one.up_weight is not other.up_weight
+
+
+def test_the_same_matrix_is_kept_once(tmp_path):
+    """By the names of what it is made of, and of the layout it is asked for in: not by where a wide matrix happens to lie."""
+    from liyab_amd.config.plan import TensorSource
+    from liyab_amd.parts.linear import product_matrix
+    from liyab_amd.weights.loader import WeightStore
+
+    w = {n: torch.randn(64, 64, generator=torch.Generator().manual_seed(i)) for i, n in enumerate("ab")}
+    store = WeightStore(w, device="cuda:0", compute_dtype=torch.float32, products="mxfp4")
+    a = product_matrix(store, TensorSource("a"), (64, 64))
+    assert product_matrix(store, TensorSource("a"), (64, 64)) is a
+    turned = product_matrix(store, TensorSource("a", layout="in_out"), (64, 64))
+    doubled = product_matrix(store, TensorSource("a"), (64, 64), (("doubled", "a"), lambda m: 2 * m))
+    joined = product_matrix(store, [TensorSource("a"), TensorSource("b")], [(64, 64)] * 2)
+    from liyab_amd.kernels.mx import Mxfp4Matrix
+
+    for got, wide in ((a, w["a"]), (turned, w["a"].t()), (doubled, 2 * w["a"]), (joined, torch.cat([w["a"], w["b"]]))):
+        assert torch.equal(got.blocks, Mxfp4Matrix.quantize(wide.contiguous().to("cuda:0")).blocks)
+    assert not store._cache and not store._derived
