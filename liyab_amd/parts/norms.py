@@ -141,10 +141,10 @@ class RMSNorm:
             ops.rmsnorm(out, x, self.weight, self.eps, rows=rows)
         return out
 
-    def mx_rows(self, x: torch.Tensor, ctx: StepContext, name: str, add: Optional[torch.Tensor] = None) -> mx.Mxfp8Rows:
-        """The norm of every row of x [n, width] in 8 bits; with `add`, x += add first."""
+    def mx_rows(self, x: torch.Tensor, ctx: StepContext, name: str) -> mx.Mxfp8Rows:
+        """The norm of every row of x [n, width] in 8 bits."""
         out = mx_place(ctx, name, x.shape[0], self.width)
-        mx.norm_mx(out, x, self.weight, self.eps, add=add, stream=x if add is not None else None)
+        mx.norm_mx(out, x, self.weight, self.eps)
         return out
 
 
