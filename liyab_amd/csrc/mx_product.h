@@ -30,7 +30,8 @@ __device__ __forceinline__ mx_bf16x8 mx_eight_of(uint32_t word, float power) {
     return mx_bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Eight numbers of a row in 8 bits as bfloat16, scale and all: three bits of mantissa and a power of two, exact.
+// Eight numbers of a row in 8 bits as bfloat16, scale and all: three bits of mantissa and a power of two, exact (where bfloat16 has their magnitude: from scales of
+// 2^-124 on all of them, and up to 2^127).
 __device__ __forceinline__ mx_bf16x8 mx_eight_of_rows(uint32_t lo, uint32_t hi, float power) {
     const mx_bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, false), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, power, true),
                     c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, false), d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, power, true);

@@ -728,3 +728,49 @@ def test_the_stream_is_what_the_norm_reads_or_lies_apart(mx, d):
         with pytest.raises(KernelError):
             mx.norm_mx(want, kw.pop("x"), w, 1e-5, **kw)
     assert not flat.any()
+
+
+@pytest.mark.parametrize("added", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("d", [33, 512, 513, 2049, 4100, 8200, 40003])
+def test_norms_next_to_borders_at_every_kernel_and_odd_widths(mx, d, added):
+    """Sums of 32 bits anywhere in a norm would put some of these values on the wrong side of a border: they lie a few 2^-26 beside one."""
+    x, add = rnd(1, d, seed=71), rnd(1, d, seed=72, dtype=added)
+    t = x.double().cpu().numpy() + add.double().cpu().numpy()
+    for centred in (False, True):
+        c = t - t.mean() if centred else t
+        w = torch.from_numpy(beside_borders(c[0], 73)).to(DEV)
+        out = empty_rows(mx, 1, d)
+        mx.norm_mx(out, x, w, 0.0, centred=centred, add=add)
+        check_rows(out, *plain_mx.quantize(c / np.sqrt((c ** 2).mean()) * w.double().cpu().numpy(), plain_mx.E4M3, 8), f"centred {centred}")
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu_tanh", "clamped"])
+@pytest.mark.parametrize("n,d", [(7, 33), (3, 514), (2, 2500), (5, 4096)])
+def test_gates_next_to_borders(mx, n, d, activation):
+    """Values within 2^-24 of a border, and further than the 1e-9 that a gate's exponential and quotient stay well below."""
+    rng = np.random.default_rng(81)
+    slope, shift, limit = 1.75, 0.5, 1024.0  # (32 bits hold these)
+    g = rng.uniform(0.5, 4.0, size=(n, d)).astype(np.float32).astype(np.float64)
+    a = plain_mx.gelu(g, activation) if activation != "clamped" else g / (1 + np.exp(-slope * g))
+    shift = shift if activation == "clamped" else 0.0
+    border = (8 + rng.integers(0, 8, size=(n, d)) + 0.5) * np.exp2(rng.integers(-3, 8, size=(n, d)) - 3.0)
+    border[:, ::32] = 400.0
+    u = (border / a - shift).astype(np.float32)
+    near = np.abs(a * (u.astype(np.float64) + shift) / border - 1) < 1e-9
+    u[near] = np.nextafter(u[near], np.float32(2000))
+    u = u.astype(np.float64)
+    out = empty_rows(mx, n, d)
+    mx.glu_mx(out, torch.from_numpy(np.concatenate([g, u], axis=1)).float().to(DEV), activation, clamp=(limit, slope, shift) if activation == "clamped" else None)
+    u = np.clip(u, -limit, limit) if activation == "clamped" else u
+    check_rows(out, *plain_mx.quantize(a * (u + shift), plain_mx.E4M3, 8), activation)
+
+
+def test_blocks_between_pieces_are_refused(mx):
+    """Blocks start on 16-byte boundaries, as the products' loads take them."""
+    from liyab_amd.errors import KernelError
+
+    flat = torch.zeros(2 * mx.BLOCK_BYTES + 16, dtype=torch.uint8, device=DEV)
+    mx.Mxfp4Matrix(flat[16:].view(2, 1, mx.BLOCK_BYTES), 32, 64)
+    for at in (1, 4, 8, 15):
+        with pytest.raises(KernelError):
+            mx.Mxfp4Matrix(flat[at:at + 2 * mx.BLOCK_BYTES].view(2, 1, mx.BLOCK_BYTES), 32, 64)
