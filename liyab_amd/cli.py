@@ -41,7 +41,7 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--ctx", type=int, default=None, help="context length (default: the model's)")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32", "bf16", "fp32"],
                     help="precision of the whole path (default bfloat16)")
-    ap.add_argument("--weights", default=None, choices=["mxfp4"], help="matrices of attention's and the feed-forwards' products in 4 bits, rounded at load (default: as --dtype says)")
+    ap.add_argument("--weights", default=None, choices=["mxfp4"], help="matrices of plain and scored attention, dense feed-forwards and selective scans in 4 bits, rounded at load; others stay (default: as --dtype says)")
     ap.add_argument("--rows", default=None, choices=["mxfp8"], help="with --weights: these products take their rows in 8 bits (default: as --dtype says)")
     ap.add_argument("--json", action="store_true", help="stdout: one JSON line after loading and one for the generation")
     ap.add_argument("--tokenize", action="store_true", help="print the prompt's token ids and exit")

@@ -56,8 +56,8 @@ enum : int { kMxPlain = 0, kMxSilu = 1, kMxGeluTanh = 2, kMxClamped = 3 };
 
 // Values next to a border of the 8-bit numbers, or of a group's scale, need more than 32 bits to fall on the right side: gates and norms are
 // computed in 64 (whose multiply-adds go at the rate of single 32-bit ones) and come to 32 rounded to odd, which no later rounding is misled by. In 32 bits
-// throughout some values of every 16 million landed on the wrong side, off by 1e-5 to 1e-4 in the 2-norm, now none (2,048 rows of 16,384: gates 54.5 us then,
-// 5.5 TB/s, and 56.0 now; norms of 2,048 rows of 4,096 19.7 and 20.4, 4.5 TB/s).
+// throughout some values of every 16 million landed on the wrong side, off by 1e-5 to 1e-4 in the 2-norm, now none (2,048 rows of 16,384: gates 54.5 us then
+// and 54.6 now, 5.5 TB/s; norms of 2,048 rows of 4,096 19.7 and 20.5, 4.5 TB/s).
 __device__ __forceinline__ float to_odd(double v) {
     const uint64_t bits = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = static_cast<uint32_t>(bits);

@@ -32,8 +32,9 @@ class EngineCore:
         caller's accounting). With neither, every request slot can reach the full context.
         `batch_invariant`: a request's bfloat16 logits have the same bits alone and in any batch
         (kernels chosen from sizes and positions only: slower; float32 is so either way).
-        `weights="mxfp4"`: the matrices of attention's and the feed-forwards' products in 4 bits, groups of 32 under a
-        power of two, rounded at load (embeddings, heads, routed experts and what recurrences read stay as they are);
+        `weights="mxfp4"`: the matrices of plain and scored attention, of dense feed-forwards and of selective scans' first and
+        last projections in 4 bits, groups of 32 under a power of two, rounded at load (latent and differential attention, other
+        recurrences, experts, routers, embeddings and heads stay as they are; a model with none of the former is refused);
         `rows="mxfp8"` with it, in bfloat16: these products take their rows in 8 bits."""
         if not torch.cuda.is_available():
             raise KernelError("no GPU is visible: this engine runs on gfx950 only and has no CPU path")

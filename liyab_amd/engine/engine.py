@@ -57,8 +57,8 @@ class Engine:
         as captured HIP graphs (a part that decides on the host from a step's values, not from
         its shape, needs this off). `batch_invariant`: every reply, greedy or seeded, is the same alone and in any batch in
         bfloat16 too, as the reference promises (include/liyab/engine.h:987-990): kernels are chosen
-        from the model's sizes and a token's position only, which costs speed. `weights="mxfp4"`, and `rows="mxfp8"` with it: the matrices of attention's and
-        the feed-forwards' products in 4 bits, their rows in 8 (`EngineCore`). `phases`: time the device per phase of the forward pass (`phases_ms()`;
+        from the model's sizes and a token's position only, which costs speed. `weights="mxfp4"`, and `rows="mxfp8"` with it: matrices of attention and
+        dense feed-forwards in 4 bits, their products' rows in 8 (`EngineCore` says which). `phases`: time the device per phase of the forward pass (`phases_ms()`;
         steps are then launched kernel by kernel, so generation is slower). `ctx`: the
         context length (default: the model's). `prefill_chunk`: the longest
         portion of a prompt in one step (the reference's 256,

@@ -43,7 +43,7 @@ class SideBySide:
         self.left_out = store.fetch(t["left_out"], (self.width,), "vector") if self.normed else None
         self.right_out = store.fetch(t["right_out"], (self.width,), "vector") if self.normed else None
         # both read the same rows: where both have one input projection and take its rows from the caller (`in_weight`,
-        # forward(..., proj=)), the two run as one product [left | right]
+        # forward(..., proj=)), the two run as one product [left | right] (not where one of them is kept in 4 bits: two products then)
         self.joint_weight = self.joint_bias = None
         if all(isinstance(getattr(p, "in_weight", None), torch.Tensor) and "proj" in p.forward.__code__.co_varnames for p in (self.left, self.right)) \
                 and self.left.in_weight.dtype == self.right.in_weight.dtype:
