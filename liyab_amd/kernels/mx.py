@@ -40,11 +40,15 @@ def _round_up(n: int, m: int) -> int:
     return -(-n // m) * m
 
 
-def _bytes(t: torch.Tensor, what: str) -> torch.Tensor:
-    """The bytes of a tensor of 8-bit elements (uint8, or one of torch's 8-bit floating-point types), rows contiguous."""
+# torch's types of what the formats hold; a tensor of another 8-bit type stands for other numbers than its bytes would be taken for
+_E4M3, _E2M1, _E8M0 = torch.float8_e4m3fn, torch.float4_e2m1fn_x2, torch.float8_e8m0fnu
+
+
+def _bytes(t: torch.Tensor, what: str, kind: torch.dtype) -> torch.Tensor:
+    """The bytes of a tensor of uint8 or of `kind`, rows contiguous."""
     _dev(t, what)
-    if t.element_size() != 1 or t.dtype in (torch.bool, torch.int8):
-        raise KernelError(f"{what} must hold bytes (uint8, float8_e4m3fn, float8_e8m0fnu), not {t.dtype}")
+    if t.dtype not in (torch.uint8, kind):
+        raise KernelError(f"{what} must be uint8 or {str(kind).replace('torch.', '')}, not {t.dtype}")
     t = t if t.dtype == torch.uint8 else t.view(torch.uint8)
     if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
         raise KernelError(f"{what} must be 2-D with contiguous rows, got shape {tuple(t.shape)} strides {t.stride()}")
@@ -98,9 +102,9 @@ class Mxfp4Matrix:
 
     @classmethod
     def pack(cls, codes: torch.Tensor, scales: torch.Tensor, width: int) -> "Mxfp4Matrix":
-        """From plain rows: codes uint8 [out, ceil(width / 2)], two numbers a byte, the first in the low half (or whole groups, [out, 16 ceil(width / 32)],
-        where what lies behind the width does not count), and scales [out, ceil(width / 32)]."""
-        codes, scales = _bytes(codes, "codes"), _bytes(scales, "scales")
+        """From plain rows: codes uint8 (or float4_e2m1fn_x2) [out, ceil(width / 2)], two numbers a byte, the first in the low half (or whole groups, [out, 16 ceil(width / 32)],
+        where what lies behind the width does not count), and scales [out, ceil(width / 32)], uint8 or float8_e8m0fnu."""
+        codes, scales = _bytes(codes, "codes", _E2M1), _bytes(scales, "scales", _E8M0)
         if width < 1 or codes.shape[1] not in (-(-width // 2), -(-width // GROUP) * (GROUP // 2)) or tuple(scales.shape) != (codes.shape[0], -(-width // GROUP)) or scales.device != codes.device:
             raise KernelError(f"a 4-bit matrix of width {width} needs codes [out, {-(-width // 2)}] or [out, {-(-width // GROUP) * (GROUP // 2)}] and scales [out, {-(-width // GROUP)}], got {tuple(codes.shape)} and {tuple(scales.shape)}")
         out = cls._empty(codes.shape[0], width, codes.device)
@@ -157,8 +161,8 @@ class Mxfp8Rows:
 
     @classmethod
     def pack(cls, codes: torch.Tensor, scales: torch.Tensor) -> "Mxfp8Rows":
-        """From plain rows: codes [n, width] (float8_e4m3fn, or their bytes) and scales [n, ceil(width / 32)] (bytes)."""
-        codes, scales = _bytes(codes, "codes"), _bytes(scales, "scales")
+        """From plain rows: codes [n, width] (float8_e4m3fn, or their bytes) and scales [n, ceil(width / 32)] (float8_e8m0fnu, or their bytes)."""
+        codes, scales = _bytes(codes, "codes", _E4M3), _bytes(scales, "scales", _E8M0)
         n, width = codes.shape
         if width < 1 or tuple(scales.shape) != (n, -(-width // GROUP)) or scales.device != codes.device:
             raise KernelError(f"rows [{n}, {width}] need scales [{n}, {-(-width // GROUP)}], got {tuple(scales.shape)}")

@@ -774,3 +774,27 @@ def test_blocks_between_pieces_are_refused(mx):
     for at in (1, 4, 8, 15):
         with pytest.raises(KernelError):
             mx.Mxfp4Matrix(flat[at:at + 2 * mx.BLOCK_BYTES].view(2, 1, mx.BLOCK_BYTES), 32, 64)
+
+
+def test_packed_numbers_are_of_the_formats_types(mx):
+    """Bytes, or torch's types of the same numbers; other 8-bit types hold other numbers in the same bytes."""
+    from liyab_amd.errors import KernelError
+
+    g = torch.Generator().manual_seed(91)
+    codes = (torch.randint(0, 126, (3, 64), generator=g, dtype=torch.uint8) + 128 * torch.randint(0, 2, (3, 64), generator=g, dtype=torch.uint8)).to(DEV)
+    four, scales = torch.randint(0, 256, (3, 32), generator=g, dtype=torch.uint8).to(DEV), torch.randint(100, 140, (3, 2), generator=g, dtype=torch.uint8).to(DEV)
+    rows = mx.Mxfp8Rows.pack(codes, scales)
+    typed = mx.Mxfp8Rows.pack(codes.view(torch.float8_e4m3fn), scales.view(torch.float8_e8m0fnu))
+    assert torch.equal(rows.codes, typed.codes) and torch.equal(rows.scales, typed.scales)
+    matrix = mx.Mxfp4Matrix.pack(four, scales, 64)
+    assert torch.equal(matrix.blocks, mx.Mxfp4Matrix.pack(four.view(torch.float4_e2m1fn_x2), scales.view(torch.float8_e8m0fnu), 64).blocks)
+    for other in (torch.float8_e5m2, torch.float8_e4m3fnuz, torch.float8_e5m2fnuz, torch.float8_e8m0fnu, torch.int8, torch.float4_e2m1fn_x2):
+        with pytest.raises(KernelError):
+            mx.Mxfp8Rows.pack(codes.view(other), scales)
+    for other in (torch.float8_e4m3fn, torch.float8_e5m2, torch.int8):
+        with pytest.raises(KernelError):
+            mx.Mxfp4Matrix.pack(four.view(other), scales, 64)
+        with pytest.raises(KernelError):
+            mx.Mxfp8Rows.pack(codes, scales.view(other))
+        with pytest.raises(KernelError):
+            mx.Mxfp4Matrix.pack(four, scales.view(other), 64)
